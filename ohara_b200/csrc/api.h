@@ -231,4 +231,56 @@ void sample_tokens(const void* logits, bool logits_bf16, int64_t row_stride, int
                    int64_t* next_input, int* step_dev, int* pos_dev, unsigned int* done,
                    float* workspace, cudaStream_t stream);
 
+// vocab_rows.cu: rows of logits over the vocabulary. Row r starts at
+// base + (r / inner) * outer_stride + (r % inner) * inner_stride (elements); its last dimension is
+// contiguous.
+struct RowsView {
+  const void* base;
+  int64_t outer_stride, inner_stride, inner;
+};
+enum class LogitType { F32, BF16, F16 };
+constexpr int kMaxAlternatives = 128;  // longest top list / teacher's list of a row
+
+struct TokenLogprobsArgs {
+  const int64_t* tokens;  // (rows) or null
+  float* logprobs;        // (rows) or null
+  float* entropy;         // (rows) or null
+  float* top_logprobs;    // (rows, top)
+  int64_t* top_tokens;    // (rows, top)
+  float4* stats;          // (rows): reference, sum (inf: row skipped), entropy
+  int64_t ignore_index;
+  float inv_temperature;
+  int vocab, top, parts;
+};
+void token_logprobs(const RowsView& view, LogitType type, TokenLogprobsArgs args, int64_t rows,
+                    cudaStream_t stream);
+
+struct DistillationArgs {
+  const float* teacher;   // (rows, top) log-probabilities
+  const int64_t* tokens;  // (rows, top), negative: no entry
+  float* loss;            // (rows)
+  float4* stats;          // (rows): reference, sum (inf: row skipped), list's log-sum or mass, outside sum
+  float inv_temperature;
+  int vocab, top, tail, parts;
+};
+void distillation_loss(const RowsView& view, LogitType type, DistillationArgs args, int64_t rows,
+                       cudaStream_t stream);
+
+// Gradient with respect to the logits of either of the two, from the `stats` that it left.
+struct VocabGradArgs {
+  const float4* stats;
+  void* out;              // (rows, out_pitch)
+  int64_t out_pitch;
+  const float* grad;          // (rows): of the log-probabilities (or null) / of the loss
+  const float* grad_entropy;  // (rows) or null
+  const float* grad_top;      // (rows, top) or null
+  const int64_t* tokens;      // (rows) targets / (rows, top) teacher's list
+  const int64_t* top_tokens;  // (rows, top) with grad_top
+  const float* teacher;       // (rows, top)
+  float inv_temperature;
+  int vocab, top, tail, parts;
+};
+void vocab_grad(const RowsView& view, LogitType type, LogitType out_type, VocabGradArgs args,
+                int64_t rows, bool distill, cudaStream_t stream);
+
 }  // namespace ob

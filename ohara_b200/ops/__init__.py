@@ -27,15 +27,19 @@ import os as _os
 _FUSE_PROJECTIONS = _os.environ.get("OHARA_FUSED_PROJECTIONS", "1") != "0"
 
 __all__ = [
+    "TokenLogprobs",
     "add_rms_norm",
     "attention",
     "bf16_weight",
+    "distillation_loss",
     "embedding",
     "fast_path",
     "linear",
     "linear_cross_entropy",
     "linear_cat",
+    "linear_distillation_loss",
     "linear_fanout",
+    "linear_token_logprobs",
     "rope_attention",
     "swiglu_cat",
     "matmul_nn",
@@ -44,6 +48,7 @@ __all__ = [
     "rms_norm",
     "rope_qk",
     "swiglu",
+    "token_logprobs",
     "check_status",
 ]
 
@@ -593,7 +598,15 @@ def embedding(ids: Tensor, table: Tensor) -> Tensor:
 
 
 # --------------------------------------------------------------------------------------------------
-# Attention (implemented in ops/attention.py) and fused linear + cross-entropy (ops/loss.py)
+# Attention (ops/attention.py), fused linear + cross-entropy (ops/loss.py), log-probabilities and
+# distillation over the vocabulary (ops/logprobs.py)
 # --------------------------------------------------------------------------------------------------
 from .attention import attention, rope_attention  # noqa: E402
+from .logprobs import (  # noqa: E402
+    TokenLogprobs,
+    distillation_loss,
+    linear_distillation_loss,
+    linear_token_logprobs,
+    token_logprobs,
+)
 from .loss import linear_cross_entropy  # noqa: E402
