@@ -39,6 +39,40 @@ constexpr float kLeastRest = 1e-6f;
 constexpr int kUnroll = 4;       // 16-byte loads in flight per thread
 constexpr int kMaxCluster = 8;   // the portable cluster size
 
+// Maximum that keeps a NaN (fmaxf drops it, and a NaN logit has to reach the top list).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Two floats in one register pair: sm_100 adds, multiplies and fuses them with one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Elements
 // ---------------------------------------------------------------------------------------------
@@ -52,6 +86,10 @@ struct Elem<float> {
   static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[4]) {
     f[0] = __uint_as_float(r.x), f[1] = __uint_as_float(r.y);
     f[2] = __uint_as_float(r.z), f[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ float highest(const uint4& r) {
+    return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)),
+                   max_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
 };
 template <>
@@ -67,6 +105,11 @@ struct Elem<__nv_bfloat16> {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+  static __device__ __forceinline__ float highest(const uint4& r) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
+  }
 };
 template <>
 struct Elem<__half> {
@@ -80,6 +123,11 @@ struct Elem<__half> {
       const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
       f[2 * i] = v.x, f[2 * i + 1] = v.y;
     }
+  }
+  static __device__ __forceinline__ float highest(const uint4& r) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
 };
 
@@ -101,13 +149,6 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 __device__ __forceinline__ void store_vec(__half* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pack_half(v[0], v[1]), pack_half(v[2], v[3]),
                                             pack_half(v[4], v[5]), pack_half(v[6], v[7]));
-}
-
-// Maximum that keeps a NaN (fmaxf drops it, and a NaN logit has to reach the top list).
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -162,55 +203,92 @@ __device__ __forceinline__ void rebase(Stats& a, float m, float c) {
   a.m = m;
 }
 
-template <Kind K>
-__device__ __forceinline__ void merge(Stats& a, Stats b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  rebase<K>(a, m, c);
-  rebase<K>(b, m, c);
-  a.s += b.s;
-  a.w += b.w;
-}
-
-// One logit, with the maximum already at or above it.
-template <Kind K>
-__device__ __forceinline__ void add_one(Stats& a, float x, float ref, float c, bool in_list = false) {
-  const float d = x - ref;
-  const float e = fast_exp2(d * c);
-  if (K == kSplit && !in_list)
-    a.w += e;
-  else
-    a.s += e;
-  // a masked logit has e = 0 and d = -inf: the clamp makes their product 0 instead of NaN
-  if (K == kEntropy) a.w = fmaf(e, fmaxf(d, -3.0e38f), a.w);
-}
+// A thread's sums over the logits it has read, even and odd elements apart.
+struct Running {
+  float m;
+  uint64_t s, w;
+};
 
 template <Kind K>
-__device__ __forceinline__ Stats warp_merge(Stats a, float c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
-    merge<K>(a, b, c);
+__device__ __forceinline__ void raise(Running& a, float m, float c) {
+  const float shift = a.m - m;
+  const float f = fast_exp2(shift * c);
+  if (f == 0.f) {  // as in `rebase`
+    const float2 s = both(a.s), w = both(a.w);
+    a.s = pair(s.x == s.x ? 0.f : s.x, s.y == s.y ? 0.f : s.y);
+    a.w = pair(w.x == w.x ? 0.f : w.x, w.y == w.y ? 0.f : w.y);
+  } else {
+    const uint64_t f2 = pair(f, f);
+    if (K == kEntropy) a.w = fma2(a.s, pair(shift, shift), a.w);
+    if (K != kSum) a.w = mul2(a.w, f2);
+    a.s = mul2(a.s, f2);
   }
+  a.m = m;
+}
+
+// The N logits of one vector, with the maximum already at or above them. `in_list` (kSplit): a bit per
+// logit. Per pair: subtract, scale, two exponentials, add (and clamp, fuse for the entropy).
+template <Kind K, int N>
+__device__ __forceinline__ void accumulate(Running& a, const float (&f)[N], float c, uint32_t in_list) {
+  const float ref = reference_of(a.m);
+  const uint64_t ref2 = pair(-ref, -ref), c2 = pair(c, c);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t d = add2(pair(f[i], f[i + 1]), ref2);
+    const float2 t = both(mul2(d, c2));
+    const float2 e = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+    if (K == kSplit) {
+      if (in_list == 0) {
+        a.w = add2(a.w, pair(e.x, e.y));
+      } else {
+        const bool x = (in_list >> i) & 1, y = (in_list >> (i + 1)) & 1;
+        a.s = add2(a.s, pair(x ? e.x : 0.f, y ? e.y : 0.f));
+        a.w = add2(a.w, pair(x ? 0.f : e.x, y ? 0.f : e.y));
+      }
+    } else {
+      a.s = add2(a.s, pair(e.x, e.y));
+    }
+    if (K == kEntropy) {
+      const float2 dd = both(d);
+      a.w = fma2(pair(e.x, e.y), pair(fmaxf(dd.x, -3.0e38f), fmaxf(dd.y, -3.0e38f)), a.w);
+    }
+  }
+}
+
+// The sums of one logit.
+template <Kind K>
+__device__ __forceinline__ Running first_of(float x, float c, bool in_list) {
+  Running a{fmaxf(x, -INFINITY), 0, 0};  // a NaN is no maximum
+  const float e = fast_exp2((x - reference_of(a.m)) * c);
+  if (K == kSplit && !in_list)
+    a.w = pair(e, 0.f);
+  else
+    a.s = pair(e, 0.f);
   return a;
 }
 
-// The CTA's statistics, in every thread of warp 0. One barrier.
-template <Kind K, int THREADS>
-__device__ __forceinline__ Stats block_merge(Stats a, float c, float4* scratch) {
-  a = warp_merge<K>(a, c);
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float4(a.m, a.s, a.w, 0.f);
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    a = Stats{-INFINITY, 0.f, 0.f};
-    if (threadIdx.x < THREADS / 32) {
-      const float4 v = scratch[threadIdx.x];
-      a = Stats{v.x, v.y, v.z};
-    }
-    a = warp_merge<K>(a, c);
-  }
+__device__ __forceinline__ Stats folded(const Running& a) {
+  const float2 s = both(a.s), w = both(a.w);
+  return Stats{a.m, s.x + s.y, w.x + w.y};
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One maximum for the warp first, so that every lane moves its sums once.
+template <Kind K>
+__device__ __forceinline__ Stats warp_merge(Stats a, float c) {
+  rebase<K>(a, warp_max(a.m), c);
+  a.s = warp_sum(a.s);
+  if (K != kSum) a.w = warp_sum(a.w);
   return a;
 }
 
@@ -247,7 +325,8 @@ __device__ __forceinline__ uint64_t block_kth(int k, int (*partial)[THREADS / 32
 // ---------------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ const T* row_of(const RowsView& v, int64_t row) {
-  const int64_t outer = row / v.inner;
+  // (a 64-bit division is sixty instructions, and most views have one leading stride)
+  const int64_t outer = row < v.inner ? 0 : row / v.inner;
   return static_cast<const T*>(v.base) + outer * v.outer_stride + (row - outer * v.inner) * v.inner_stride;
 }
 
@@ -298,7 +377,7 @@ __device__ __forceinline__ void store_cluster_i32(uint32_t addr, int v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// The statistics of all CTAs of the cluster, in warp 0 of the first one. `slots` is a shared array
+// The statistics of all CTAs of the cluster, in every warp of the first one. `slots` is a shared array
 // of kMaxCluster entries; the cluster barrier also publishes what the caller stored to the first CTA
 // before the call, and no CTA leaves before every store to the first one has landed.
 template <Kind K>
@@ -307,28 +386,41 @@ __device__ __forceinline__ Stats cluster_merge(Stats mine, float c, float4* slot
   cluster_arrive();
   cluster_wait();
   Stats a{-INFINITY, 0.f, 0.f};
-  if (part == 0 && threadIdx.x < 32) {
-    if (threadIdx.x < parts) {
-      const float4 v = slots[threadIdx.x];
-      a = Stats{v.x, v.y, v.z};
-    }
-    a = warp_merge<K>(a, c);
+  const int lane = threadIdx.x & 31;
+  if (part == 0 && lane < parts) {
+    const float4 v = slots[lane];
+    a = Stats{v.x, v.y, v.z};
   }
-  return a;
+  return warp_merge<K>(a, c);
 }
 
 // ---------------------------------------------------------------------------------------------
 // Token log-probabilities
 // ---------------------------------------------------------------------------------------------
+// The top K of a row without a second pass over it. Every lane remembers its best vector so far (its
+// maximum and position); the j-th best of a warp's 32 lanes, and the i-th best of those over the warps
+// (i j >= K), is a vector that at least K distinct vectors reach, so no element of a vector below
+// that bound can be among the K. Vectors that reach it are noted (their position, in a list of the
+// warp), the bound is taken again after 1, 2, 4, ... sweeps, and at the end the noted vectors are read
+// once more (from L2) against the last bound. For random logits that leaves about 1.75 K elements, which
+// are ordered by counting. The order of vectors is (maximum, then position), so ties - a row of one
+// value, masked logits - do not flood the lists. A row that floods them all the same (in ascending
+// order, say) goes through `block_kth` over the whole slice.
 template <int THREADS>
 struct TopShared {
-  static constexpr int kCap = THREADS >= 256 ? 8 * THREADS : 16 * THREADS;
-  uint64_t codes[kCap];                          // candidates of this CTA's slice
-  uint64_t merged[kMaxCluster][kMaxAlternatives];  // sorted lists of the cluster's CTAs
+  static constexpr int kWarps = THREADS / 32;
+  static constexpr int kHits = THREADS == 512 ? 128 : 512;  // noted vectors of a warp
+  static constexpr int kCap = THREADS == 128 ? 1024 : (THREADS == 256 ? 2048 : 2560);
+  uint64_t codes[kCap];  // elements that reach the last bound
+  uint32_t hits[kWarps][kHits];
+  uint64_t bound[kWarps];  // of each warp, read by the others without a barrier: none ever gets invalid
+  int partial[2][kWarps];
+  int count, overflow;
+};
+// What joins the CTAs of a cluster (the 512-thread shape).
+struct ClusterLists {
+  uint64_t merged[kMaxCluster][kMaxAlternatives];
   int merged_count[kMaxCluster];
-  uint64_t sorted[kMaxAlternatives];
-  int partial[2][THREADS / 32];
-  int count;
 };
 struct NoShared {
   int unused;
@@ -343,7 +435,7 @@ __device__ __forceinline__ void push(TopShared<THREADS>& sh, uint64_t code) {
 
 // Cuts the candidate list down to the `k` largest (all of them if there are fewer).
 template <int THREADS>
-__device__ __forceinline__ uint64_t keep_largest(TopShared<THREADS>& sh, int k) {
+__device__ __forceinline__ void keep_largest(TopShared<THREADS>& sh, int k) {
   constexpr int kPer = TopShared<THREADS>::kCap / THREADS;
   const int n = sh.count;
   uint64_t mine[kPer];
@@ -365,25 +457,119 @@ __device__ __forceinline__ uint64_t keep_largest(TopShared<THREADS>& sh, int k) 
   for (int i = 0; i < kPer; ++i)
     if (mine[i] >= least) push<THREADS>(sh, mine[i]);
   __syncthreads();
-  return least;
+}
+
+// A vector's code: its maximum, then its position, ascending positions last. 16-bit logits need 16 bits
+// for the maximum, which leaves 16 of a register for the position (in units of 2^shift vectors, 1 for
+// vocabularies below 2^19): half the instructions of the general form. Two lanes whose codes are then
+// equal only make the bound a little weaker.
+template <typename T>
+struct VectorCode {
+  using Code = uint64_t;
+  static __device__ __forceinline__ int shift_for(int) { return 0; }
+  static __device__ __forceinline__ Code make(float x, int at) { return rank_code(x, (uint32_t)at); }
+  static __device__ __forceinline__ float value(Code c) { return code_value(c); }
+  static __device__ __forceinline__ int at(Code c) { return (int)code_index(c); }
+};
+__device__ __forceinline__ int code_shift16(int vecs) { return max(0, 16 - __clz(vecs)); }
+template <>
+struct VectorCode<__nv_bfloat16> {
+  using Code = uint32_t;
+  static __device__ __forceinline__ int shift_for(int vecs) { return code_shift16(vecs); }
+  static __device__ __forceinline__ Code make(float x, int at) {
+    return (static_cast<uint32_t>(rank_code(x, 0) >> 32) & 0xffff0000u) | (0xffffu - at);
+  }
+  static __device__ __forceinline__ float value(Code c) {
+    const uint32_t key = c >> 16;
+    if (key == 0xffffu) return __uint_as_float(0x7fffffffu);
+    return __uint_as_float(((key & 0x8000u) ? (key & 0x7fffu) : (~key & 0xffffu)) << 16);
+  }
+  static __device__ __forceinline__ int at(Code c) { return 0xffff - (int)(c & 0xffffu); }
+};
+template <>
+struct VectorCode<__half> {
+  using Code = uint32_t;
+  static __device__ __forceinline__ int shift_for(int vecs) { return code_shift16(vecs); }
+  static __device__ __forceinline__ Code make(float x, int at) {
+    const uint32_t b = __half_as_ushort(__float2half_rn(x + 0.f));  // exact: x was a half
+    uint32_t key = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+    if (x != x) key = 0xffffu;
+    return (key << 16) | (0xffffu - at);
+  }
+  static __device__ __forceinline__ float value(Code c) {
+    const uint32_t key = c >> 16;
+    if (key == 0xffffu) return __uint_as_float(0x7fffffffu);
+    const uint16_t b = (uint16_t)((key & 0x8000u) ? (key & 0x7fffu) : (~key & 0xffffu));
+    return __half2float(__ushort_as_half(b));
+  }
+  static __device__ __forceinline__ int at(Code c) { return 0xffff - (int)(c & 0xffffu); }
+};
+
+// The n-th largest of the lanes' codes (0 where there are fewer), and the least.
+__device__ __forceinline__ uint64_t warp_nth(uint64_t code, int n) {
+  uint32_t hi = static_cast<uint32_t>(code >> 32), lo = static_cast<uint32_t>(code);
+  uint32_t h = 0, l = 0;
+  for (int i = 0; i < n; ++i) {
+    h = __reduce_max_sync(0xffffffffu, hi);
+    l = __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
+    if (hi == h && lo == l) hi = lo = 0;
+  }
+  return (static_cast<uint64_t>(h) << 32) | l;
+}
+__device__ __forceinline__ uint32_t warp_nth(uint32_t code, int n) {
+  uint32_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    most = __reduce_max_sync(0xffffffffu, code);
+    if (code == most) code = 0;
+  }
+  return most;
+}
+__device__ __forceinline__ uint64_t warp_least(uint64_t code) {
+  const uint32_t hi = static_cast<uint32_t>(code >> 32), lo = static_cast<uint32_t>(code);
+  const uint32_t h = __reduce_min_sync(0xffffffffu, hi);
+  const uint32_t l = __reduce_min_sync(0xffffffffu, hi == h ? lo : 0xffffffffu);
+  return (static_cast<uint64_t>(h) << 32) | l;
+}
+__device__ __forceinline__ uint32_t warp_least(uint32_t code) {
+  return __reduce_min_sync(0xffffffffu, code);
+}
+
+// How the bound for the K best is put together: the `per_warp`-th best lane of every warp, then the
+// `of_warps`-th best of those.
+struct BoundPlan {
+  int per_warp, of_warps;
+};
+template <int THREADS>
+__device__ __forceinline__ BoundPlan bound_plan(int top) {
+  constexpr int kWarps = THREADS / 32;
+  const int per_warp = (top + kWarps - 1) / kWarps;
+  return BoundPlan{per_warp, (top + per_warp - 1) / per_warp};
+}
+template <int WARPS, typename Code>
+__device__ __forceinline__ Code joint_bound(const volatile Code* bound, const BoundPlan& plan) {
+  const int lane = threadIdx.x & 31;
+  if (plan.of_warps == WARPS) return warp_least(lane < WARPS ? bound[lane] : ~Code(0));
+  return warp_nth(lane < WARPS ? bound[lane] : Code(0), plan.of_warps);
 }
 
 template <typename T, int THREADS, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, TOP ? (THREADS == 512 ? 2 : 1280 / THREADS) : (THREADS == 512 ? 3 : 1792 / THREADS))
 token_logprobs_kernel(const RowsView view, const TokenLogprobsArgs p) {
   constexpr int N = Elem<T>::kN;
-  using Shared = std::conditional_t<TOP, TopShared<THREADS>, NoShared>;
-  __shared__ Shared sh;
-  __shared__ float4 scratch[THREADS / 32];
-  __shared__ float4 slots[kMaxCluster];
-  const int parts = p.parts;
+  constexpr int kWarps = THREADS / 32;
+  constexpr bool CLUSTER = THREADS == 512;
+  constexpr Kind K = ENTROPY ? kEntropy : kSum;
+  __shared__ std::conditional_t<TOP, TopShared<THREADS>, NoShared> sh;
+  __shared__ std::conditional_t<TOP && CLUSTER, ClusterLists, NoShared> joined;
+  __shared__ float4 scratch[kWarps];
+  __shared__ float4 slots[CLUSTER ? kMaxCluster : 1];
+  const int parts = CLUSTER ? p.parts : 1;
   const int part = parts > 1 ? (int)cluster_cta_rank() : 0;
   const int64_t row = parts > 1 ? (int64_t)(blockIdx.x / parts) : (int64_t)blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vocab = p.vocab;
   const int top = p.top;
   const float c = p.inv_temperature * kLog2e;
-  constexpr Kind K = ENTROPY ? kEntropy : kSum;
 
   const int64_t token = p.tokens != nullptr ? p.tokens[row] : 0;
   if (p.tokens != nullptr && token == p.ignore_index) {
@@ -409,99 +595,145 @@ token_logprobs_kernel(const RowsView view, const TokenLogprobsArgs p) {
   if (part == 0 && tid == 0 && p.logprobs != nullptr && token >= 0 && token < vocab)
     target = Elem<T>::load(x + token);
 
-  Stats st{-INFINITY, 0.f, 0.f};
+  Running run{-INFINITY, 0, 0};
   const int edge = edge_index(sl, vocab, part);
   float edge_x = -INFINITY;
   if (edge >= 0) {
     edge_x = Elem<T>::load(x + edge);
-    st.m = fmaxf(st.m, edge_x);
-    add_one<K>(st, edge_x, reference_of(st.m), c);
+    run = first_of<K>(edge_x, c, false);
   }
   const uint4* body = reinterpret_cast<const uint4*>(x + sl.head);
-  uint64_t least = 1;         // candidates have to reach this code
-  float least_x = -INFINITY;  // its value, for the first test of a whole vector
-  bool overflow = false;
+
+  // the lane's best vector (NaN aside: that reaches every bound), the bound, and how many vectors
+  // the warp has noted
+  float best = -INFINITY, least_x = -INFINITY;
+  int best_at = -1, least_at = 0x7fffffff, noted = 0, refresh_at = 0x7fffffff;
+  const BoundPlan plan = bound_plan<THREADS>(top);
+  using V = VectorCode<T>;
+  using Code = typename V::Code;
+  const int shift = V::shift_for(sl.v1);
+  auto publish_bound = [&] {
+    if constexpr (TOP) {
+      const Code b = warp_nth(best_at < 0 ? Code(0) : V::make(best, best_at >> shift), plan.per_warp);
+      if (lane == 0) reinterpret_cast<volatile Code*>(sh.bound)[warp] = b;
+    }
+  };
+  auto take_bound = [&] {
+    if constexpr (TOP) {
+      const Code b = joint_bound<kWarps>(reinterpret_cast<const volatile Code*>(sh.bound), plan);
+      least_x = b == 0 ? -INFINITY : V::value(b);
+      least_at = b == 0 ? 0x7fffffff : (((V::at(b) + 1) << shift) - 1);
+    }
+  };
   if constexpr (TOP) {
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
+    if (tid == 0) sh.count = sh.overflow = 0;
   }
-  bool first = true;
-  // every thread takes part in every sweep (they hold barriers), also in one that is empty for it
-  for (int base = sl.v0; base < sl.v1 || (TOP && first); base += THREADS * kUnroll) {
+  int sweep = 0;
+  // kUnroll vectors per thread; a full sweep has all of them, which spares the tests
+  auto one_sweep = [&](int base, auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    auto there = [&](int u) { return FULL || base + u * THREADS + tid < sl.v1; };
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int v = base + u * THREADS + tid;
-      if (v < sl.v1) raw[u] = body[v];
-    }
+    for (int u = 0; u < kUnroll; ++u)
+      if (there(u)) raw[u] = body[base + u * THREADS + tid];
     float high[kUnroll];  // NaN-keeping maximum of each vector
+    float sweep_high = -INFINITY;
+    bool nan = false;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      high[u] = -INFINITY;
-      if (base + u * THREADS + tid >= sl.v1) continue;
+      high[u] = there(u) ? Elem<T>::highest(raw[u]) : -INFINITY;
+      sweep_high = fmaxf(sweep_high, high[u]);
+      if (TOP) nan |= high[u] != high[u];
+    }
+    if (sweep_high > run.m) raise<K>(run, sweep_high, c);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (!there(u)) continue;
       float f[N];
       Elem<T>::unpack(raw[u], f);
-      float vm = f[0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) vm = TOP ? max_nan(vm, f[i]) : fmaxf(vm, f[i]);
-      high[u] = vm;
-      if (vm > st.m) rebase<K>(st, vm, c);
-      const float ref = reference_of(st.m);
-#pragma unroll
-      for (int i = 0; i < N; ++i) add_one<K>(st, f[i], ref, c);
+      accumulate<K>(run, f, c, 0);
     }
     if constexpr (TOP) {
-      if (first) {
-        // The k-th largest of the threads' own maxima is a bound that at least k elements reach.
-        uint64_t best = edge >= 0 ? rank_code(edge_x, edge) : 0;
+      if (sweep == 0 && there(0)) best_at = base + tid;  // also if that is -inf
+      if (sweep_high > best) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (high[u] > best) {
+            best = high[u];
+            best_at = base + u * THREADS + tid;
+          }
+        }
+      }
+      // after 1, 2, 4, ... sweeps, and when many vectors were noted since the last time
+      if ((sweep & (sweep + 1)) == 0 || noted >= refresh_at) {
+        publish_bound();
+        if (sweep == 0) __syncthreads(); else __syncwarp();
+        take_bound();
+        refresh_at = noted + 128;
+      }
+      if (__any_sync(0xffffffffu, nan || !(sweep_high < least_x))) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
           const int v = base + u * THREADS + tid;
-          if (v >= sl.v1) continue;
-          float f[N];
-          Elem<T>::unpack(raw[u], f);
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const uint64_t code = rank_code(f[i], sl.head + v * N + i);
-            best = code > best ? code : best;
-          }
+          const bool hit = there(u) && !(high[u] < least_x) && (high[u] != least_x || v <= least_at);
+          const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+          if (mask == 0) continue;
+          const int at = noted + __popc(mask & ((1u << lane) - 1));
+          if (hit && at < TopShared<THREADS>::kHits) sh.hits[warp][at] = (uint32_t)v;
+          noted += __popc(mask);
         }
-        least = block_kth<THREADS>(top, sh.partial, [&](uint64_t t) { return best >= t ? 1 : 0; });
-        least_x = least == 1 ? -INFINITY : code_value(least);
-        if (edge >= 0 && rank_code(edge_x, edge) >= least) push<THREADS>(sh, rank_code(edge_x, edge));
       }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int v = base + u * THREADS + tid;
-        if (v >= sl.v1 || high[u] < least_x) continue;
+      ++sweep;
+    }
+  };
+  int base = sl.v0;
+  for (; base + THREADS * kUnroll <= sl.v1; base += THREADS * kUnroll)
+    one_sweep(base, std::true_type{});
+  // (a first sweep also where it is empty: it holds a barrier)
+  if (base < sl.v1 || (TOP && sweep == 0)) one_sweep(base, std::false_type{});
+
+  // ---- statistics of the CTA (in every warp) and the last bound: one barrier --------------------
+  Stats all = warp_merge<K>(folded(run), c);
+  if (lane == 0) scratch[warp] = make_float4(all.m, all.s, all.w, 0.f);
+  publish_bound();
+  if constexpr (TOP) {
+    if (lane == 0 && noted > TopShared<THREADS>::kHits) sh.overflow = 1;
+  }
+  __syncthreads();
+  all = Stats{-INFINITY, 0.f, 0.f};
+  if (lane < kWarps) {
+    const float4 v = scratch[lane];
+    all = Stats{v.x, v.y, v.z};
+  }
+  all = warp_merge<K>(all, c);
+
+  int found = 0;  // elements in `codes`, of which the `top` largest are the slice's list
+  if constexpr (TOP) {
+    take_bound();
+    const uint64_t edge_code = edge >= 0 ? rank_code(edge_x, edge) : 0;
+    if (sh.overflow == 0) {
+      // an element reaches the bound if its vector could have: the last place of the bound's vector
+      const uint64_t least =
+          least_at >= sl.v1 ? (least_x == -INFINITY ? 1 : rank_code(least_x, vocab))
+                            : rank_code(least_x, sl.head + least_at * N + N - 1);
+      for (int i = lane; i < noted; i += 32) {
+        const int v = (int)sh.hits[warp][i];
         float f[N];
-        Elem<T>::unpack(raw[u], f);
+        Elem<T>::unpack(body[v], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint64_t code = rank_code(f[i], sl.head + v * N + i);
+        for (int q = 0; q < N; ++q) {
+          if (f[q] < least_x) continue;
+          const uint64_t code = rank_code(f[q], sl.head + v * N + q);
           if (code >= least) push<THREADS>(sh, code);
         }
       }
-      __syncthreads();
-      const int n = sh.count;
-      __syncthreads();
-      if (n > TopShared<THREADS>::kCap) {
-        overflow = true;
-        if (tid == 0) sh.count = 0;  // found again below
-        __syncthreads();
-      } else if (n > TopShared<THREADS>::kCap / 2) {
-        least = keep_largest<THREADS>(sh, top);
-        least_x = code_value(least);
-      }
+      if (edge_code >= least) push<THREADS>(sh, edge_code);
     }
-    first = false;
-  }
-
-  if constexpr (TOP) {
-    if (overflow) {
-      // More elements of one sweep pass the bound than the list holds (rows in ascending order and
-      // the like): find the k-th largest of the slice by counting, which reads it once per bit.
-      const uint64_t edge_code = edge >= 0 ? rank_code(edge_x, edge) : 0;
+    __syncthreads();
+    if (sh.overflow != 0 || sh.count > TopShared<THREADS>::kCap) {
+      // the lists did not hold: the k-th largest of the slice by counting, which reads it once per bit
+      __syncthreads();
       auto each = [&](auto&& f) {
         for (int v = sl.v0 + tid; v < sl.v1; v += THREADS) {
           float e[N];
@@ -511,7 +743,7 @@ token_logprobs_kernel(const RowsView view, const TokenLogprobsArgs p) {
         }
         if (edge >= 0) f(edge_code);
       };
-      least = block_kth<THREADS>(top, sh.partial, [&](uint64_t t) {
+      const uint64_t least = block_kth<THREADS>(top, sh.partial, [&](uint64_t t) {
         int n = 0;
         each([&](uint64_t code) { n += code >= t ? 1 : 0; });
         return n;
@@ -522,32 +754,38 @@ token_logprobs_kernel(const RowsView view, const TokenLogprobsArgs p) {
         if (code >= least) push<THREADS>(sh, code);
       });
       __syncthreads();
-    } else if (sh.count > top) {
+    } else if (sh.count > 256) {  // beyond that, ordering by counting costs more
       keep_largest<THREADS>(sh, top);
     }
-    // order the survivors by counting the larger ones
-    const int n = sh.count;
-    if (tid < n) {
-      const uint64_t mine = sh.codes[tid];
-      int larger = 0;
-      for (int i = 0; i < n; ++i) larger += sh.codes[i] > mine ? 1 : 0;
-      sh.sorted[larger] = mine;
-    }
-    __syncthreads();
+    found = sh.count;
   }
 
-  Stats all = block_merge<K, THREADS>(st, c, scratch);
-  if (parts > 1) {
-    cluster_wait();  // every CTA of the cluster has started
+  // Calls f(place, code) for the `top` largest candidates, places by counting the larger ones.
+  auto ordered = [&](auto&& f) {
     if constexpr (TOP) {
-      const int n = sh.count;
-      if (tid == 0) store_cluster_i32(map_to_cta(smem_u32(&sh.merged_count[part]), 0), n);
-      if (tid < n)
-        store_cluster_u64(map_to_cta(smem_u32(&sh.merged[part][tid]), 0), sh.sorted[tid]);
+      for (int e = tid; e < found; e += THREADS) {
+        const uint64_t mine = sh.codes[e];
+        int larger = 0;
+        for (int i = 0; i < found; ++i) larger += sh.codes[i] > mine ? 1 : 0;
+        if (larger < top) f(larger, mine);
+      }
     }
-    all = cluster_merge<K>(all, c, slots, part, parts);
-    if (part != 0) return;
+  };
+  if constexpr (CLUSTER) {
+    if (parts > 1) {
+      cluster_wait();  // every CTA of the cluster has started
+      if constexpr (TOP) {
+        if (tid == 0)
+          store_cluster_i32(map_to_cta(smem_u32(&joined.merged_count[part]), 0), min(found, top));
+        ordered([&](int place, uint64_t code) {
+          store_cluster_u64(map_to_cta(smem_u32(&joined.merged[part][place]), 0), code);
+        });
+      }
+      all = cluster_merge<K>(all, c, slots, part, parts);
+      if (part != 0) return;
+    }
   }
+
   // ---- the row's results, by the (first) CTA --------------------------------------------------
   const float ref = reference_of(all.m);
   const float log_s = logf(all.s);
@@ -557,31 +795,28 @@ token_logprobs_kernel(const RowsView view, const TokenLogprobsArgs p) {
     const float h = log_s - all.w * p.inv_temperature / all.s;
     if (ENTROPY) p.entropy[row] = h;
     p.stats[row] = make_float4(ref, all.s, ENTROPY ? h : 0.f, 0.f);
-    scratch[0] = make_float4(ref, log_s, 0.f, 0.f);
   }
   if constexpr (TOP) {
-    __syncthreads();
-    const float r = scratch[0].x, ls = scratch[0].y;
     auto emit = [&](int place, uint64_t code) {
       if (place >= top) return;
-      p.top_logprobs[row * top + place] = fmaf(code_value(code) - r, p.inv_temperature, -ls);
+      p.top_logprobs[row * top + place] = fmaf(code_value(code) - ref, p.inv_temperature, -log_s);
       p.top_tokens[row * top + place] = (int64_t)code_index(code);
     };
     if (parts == 1) {
-      if (tid < top) emit(tid, sh.sorted[tid]);
-    } else {
+      ordered(emit);
+    } else if constexpr (CLUSTER) {
       // an entry's place: its place in its own list plus the larger entries of each other list
       for (int e = tid; e < parts * kMaxAlternatives; e += THREADS) {
         const int from = e / kMaxAlternatives, i = e - from * kMaxAlternatives;
-        if (i >= sh.merged_count[from]) continue;
-        const uint64_t code = sh.merged[from][i];
+        if (i >= joined.merged_count[from]) continue;
+        const uint64_t code = joined.merged[from][i];
         int place = i;
         for (int other = 0; other < parts; ++other) {
           if (other == from) continue;
-          int lo = 0, hi = sh.merged_count[other];
+          int lo = 0, hi = joined.merged_count[other];
           while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (sh.merged[other][mid] > code) lo = mid + 1; else hi = mid;
+            if (joined.merged[other][mid] > code) lo = mid + 1; else hi = mid;
           }
           place += lo;
         }
@@ -604,16 +839,8 @@ __device__ __forceinline__ float block_sum(float v, float* scratch, int warps) {
   for (int i = 0; i < warps; ++i) total += scratch[i];
   return total;
 }
-__device__ __forceinline__ float block_max(float v, float* scratch, int warps) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float total = scratch[0];
-  for (int i = 1; i < warps; ++i) total = fmaxf(total, scratch[i]);
-  return total;
-}
+// A lane's share of the teacher's list: entries lane, lane + 32, ...
+constexpr int kEntriesPerLane = kMaxAlternatives / 32;
 
 // One bit per logit of the slice marks the listed tokens, a byte per 16-byte vector, so that the sum
 // over the others is formed without a subtraction (1 - sum of the listed q would cancel away exactly
@@ -622,31 +849,27 @@ template <typename T, int THREADS, bool TAIL>
 __global__ void __launch_bounds__(THREADS)
 distillation_kernel(const RowsView view, const DistillationArgs p) {
   constexpr int N = Elem<T>::kN;
-  extern __shared__ uint32_t marks[];
-  __shared__ float4 scratch[THREADS / 32];
-  __shared__ float4 slots[kMaxCluster];
-  __shared__ float reduce[THREADS / 32];
-  __shared__ int64_t listed[kMaxAlternatives];
-  const int parts = p.parts;
+  constexpr int kWarps = THREADS / 32;
+  constexpr bool CLUSTER = THREADS == 512;
+  constexpr Kind K = TAIL ? kSplit : kSum;
+  extern __shared__ __align__(16) uint8_t marks[];
+  __shared__ float4 scratch[kWarps];
+  __shared__ float4 slots[CLUSTER ? kMaxCluster : 1];
+  const int parts = CLUSTER ? p.parts : 1;
   const int part = parts > 1 ? (int)cluster_cta_rank() : 0;
   const int64_t row = parts > 1 ? (int64_t)(blockIdx.x / parts) : (int64_t)blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vocab = p.vocab;
   const float c = p.inv_temperature * kLog2e;
-  constexpr Kind K = TAIL ? kSplit : kSum;
   const T* x = row_of<T>(view, row);
   const Slice sl = slice_of(x, vocab, part, parts);
+  const int64_t* tokens = p.tokens + row * p.top;
+  const float* teacher = p.teacher + row * p.top;
 
-  // ---- the teacher's entries, one per thread ---------------------------------------------------
-  int64_t token = -1;
-  float value = -INFINITY;
-  if (tid < p.top) {
-    token = p.tokens[row * p.top + tid];
-    value = p.teacher[row * p.top + tid];
-    if (token < 0) value = -INFINITY;
-  }
-  const bool counts = TAIL ? token >= 0 : value != -INFINITY;
-  if (__syncthreads_count(counts) == 0) {  // an empty list teaches nothing: the row is not read
+  // ---- does the list teach anything? (every warp looks for itself) ------------------------------
+  bool counts = false;
+  for (int k = lane; k < p.top; k += 32) counts |= tokens[k] >= 0 && (TAIL || teacher[k] != -INFINITY);
+  if (!__any_sync(0xffffffffu, counts)) {  // an empty list: the row is not read
     if (part == 0 && tid == 0) {
       p.loss[row] = 0.f;
       p.stats[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
@@ -654,97 +877,124 @@ distillation_kernel(const RowsView view, const DistillationArgs p) {
     return;
   }
   if (parts > 1) cluster_arrive();
-  const bool inside = token >= 0 && token < vocab;
-  float picked = __uint_as_float(0x7fffffffu);  // a token outside the vocabulary: NaN
-  if (inside && part == 0) picked = Elem<T>::load(x + token);
   if (TAIL) {
-    for (int i = tid; i < (sl.v1 - sl.v0 + 3) / 4; i += THREADS) marks[i] = 0;
-    if (tid < p.top) listed[tid] = token;
+    const int bytes = sl.v1 - sl.v0;
+    for (int i = tid; i < (bytes + 15) / 16; i += THREADS)
+      reinterpret_cast<uint4*>(marks)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (inside && token >= sl.head && token < sl.tail_begin) {
-      const int v = ((int)token - sl.head) / N;
-      const int bit = ((int)token - sl.head) - v * N;
-      if (v >= sl.v0 && v < sl.v1)
-        atomicOr(&marks[(v - sl.v0) >> 2], 1u << (8 * ((v - sl.v0) & 3) + bit));
+    if (warp == 0) {
+      for (int k = lane; k < p.top; k += 32) {
+        const int64_t token = tokens[k];
+        if (token < sl.head || token >= sl.tail_begin) continue;
+        const int v = ((int)token - sl.head) / N;
+        const int bit = ((int)token - sl.head) - v * N;
+        if (v >= sl.v0 && v < sl.v1)
+          atomicOr(reinterpret_cast<uint32_t*>(marks) + ((v - sl.v0) >> 2),
+                   1u << (8 * ((v - sl.v0) & 3) + bit));
+      }
     }
     __syncthreads();
   }
-  const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
+  // the first warp keeps the entries for the end: their logits arrive while the row passes
+  int64_t token[kEntriesPerLane];
+  float value[kEntriesPerLane], picked[kEntriesPerLane];
+#pragma unroll
+  for (int i = 0; i < kEntriesPerLane; ++i) {
+    const int k = lane + 32 * i;
+    token[i] = -1;
+    value[i] = -INFINITY;
+    picked[i] = __uint_as_float(0x7fffffffu);  // a token outside the vocabulary: NaN
+    if (warp == 0 && part == 0 && k < p.top) {
+      token[i] = tokens[k];
+      if (token[i] >= 0) value[i] = teacher[k];
+      if (token[i] >= 0 && token[i] < vocab) picked[i] = Elem<T>::load(x + token[i]);
+    }
+  }
 
   // ---- one pass over the logits ----------------------------------------------------------------
-  Stats st{-INFINITY, 0.f, 0.f};
+  Running run{-INFINITY, 0, 0};
   const int edge = edge_index(sl, vocab, part);
   if (edge >= 0) {
-    const float f = Elem<T>::load(x + edge);
     bool in_list = false;
     if (TAIL)
-      for (int k = 0; k < p.top; ++k) in_list |= listed[k] == edge;
-    st.m = fmaxf(st.m, f);
-    add_one<K>(st, f, reference_of(st.m), c, in_list);
+      for (int k = 0; k < p.top; ++k) in_list |= tokens[k] == edge;
+    run = first_of<K>(Elem<T>::load(x + edge), c, in_list);
   }
   const uint4* body = reinterpret_cast<const uint4*>(x + sl.head);
-  for (int base = sl.v0 + tid; base < sl.v1; base += THREADS * kUnroll) {
+  auto one_sweep = [&](int base, auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    auto there = [&](int u) { return FULL || base + u * THREADS + tid < sl.v1; };
     uint4 raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (base + u * THREADS < sl.v1) raw[u] = body[base + u * THREADS];
+      if (there(u)) raw[u] = body[base + u * THREADS + tid];
+    float high = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (there(u)) high = fmaxf(high, Elem<T>::highest(raw[u]));
+    if (high > run.m) raise<K>(run, high, c);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int v = base + u * THREADS;
-      if (v >= sl.v1) continue;
+      if (!there(u)) continue;
       float f[N];
       Elem<T>::unpack(raw[u], f);
-      float vm = f[0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) vm = fmaxf(vm, f[i]);
-      if (vm > st.m) rebase<K>(st, vm, c);
-      const float ref = reference_of(st.m);
-      const uint32_t in_list = TAIL ? mark[v - sl.v0] : 0;
-      if (in_list == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) add_one<K>(st, f[i], ref, c);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) add_one<K>(st, f[i], ref, c, (in_list >> i) & 1);
-      }
+      accumulate<K>(run, f, c, TAIL ? marks[base + u * THREADS + tid - sl.v0] : 0);
+    }
+  };
+  int base = sl.v0;
+  for (; base + THREADS * kUnroll <= sl.v1; base += THREADS * kUnroll)
+    one_sweep(base, std::true_type{});
+  if (base < sl.v1) one_sweep(base, std::false_type{});
+  Stats all = warp_merge<K>(folded(run), c);
+  if (lane == 0) scratch[warp] = make_float4(all.m, all.s, all.w, 0.f);
+  __syncthreads();
+  all = Stats{-INFINITY, 0.f, 0.f};
+  if (lane < kWarps) {
+    const float4 v = scratch[lane];
+    all = Stats{v.x, v.y, v.z};
+  }
+  all = warp_merge<K>(all, c);
+  if constexpr (CLUSTER) {
+    if (parts > 1) {
+      cluster_wait();  // every CTA of the cluster has started
+      all = cluster_merge<K>(all, c, slots, part, parts);
     }
   }
-  Stats all = block_merge<K, THREADS>(st, c, scratch);
-  if (parts > 1) {
-    cluster_wait();
-    all = cluster_merge<K>(all, c, slots, part, parts);
-    if (part != 0) return;
-  }
+  if (part != 0 || warp != 0) return;
 
-  // ---- the row's loss, by the (first) CTA -------------------------------------------------------
-  if (tid == 0) slots[0] = make_float4(reference_of(all.m), all.s, all.w, 0.f);
-  __syncthreads();
-  const float ref = slots[0].x, outside = slots[0].z;
-  const float total = TAIL ? slots[0].y + outside : slots[0].y;
+  // ---- the row's loss, by one warp ---------------------------------------------------------------
+  const float ref = reference_of(all.m), outside = all.w;
+  const float total = TAIL ? all.s + outside : all.s;
   const float log_s = logf(total);
-  float weight, log_weight, extra = 0.f;
-  if (TAIL) {
-    weight = expf(value);
-    log_weight = value;
-  } else {
-    const float high = block_max(value, reduce, THREADS / 32);
-    const float mass = block_sum(expf(value - high), reduce, THREADS / 32);
-    weight = expf(value - high) / mass;
-    log_weight = value - high - logf(mass);
-    extra = high + logf(mass);
+  float list_log = 0.f;  // log-sum of the list, which renormalises it
+  if (!TAIL) {
+    float high = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) high = fmaxf(high, value[i]);
+    high = warp_max(high);
+    float mass = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEntriesPerLane; ++i) mass += expf(value[i] - high);
+    list_log = high + logf(warp_sum(mass));
   }
-  const float term =
-      weight == 0.f ? 0.f : weight * (log_weight - fmaf(picked - ref, p.inv_temperature, -log_s));
-  float loss = block_sum(term, reduce, THREADS / 32);
+  float loss = 0.f, mass = 0.f;
+#pragma unroll
+  for (int i = 0; i < kEntriesPerLane; ++i) {
+    const float log_p = value[i] - list_log;
+    const float weight = expf(log_p);
+    mass += weight;
+    if (weight != 0.f) loss += weight * (log_p - fmaf(picked[i] - ref, p.inv_temperature, -log_s));
+  }
+  loss = warp_sum(loss);
+  mass = warp_sum(mass);
   if (TAIL) {
-    extra = block_sum(weight, reduce, THREADS / 32);
-    const float rest = 1.f - extra;
+    const float rest = 1.f - mass;
     if (!(rest <= kLeastRest)) loss += rest * (logf(rest) - (logf(outside) - log_s));
   }
-  if (tid == 0) {
+  if (lane == 0) {
     p.loss[row] = loss;
     // a NaN loss has a NaN gradient, also where it comes from a token outside the vocabulary
-    p.stats[row] = make_float4(ref, loss == loss ? total : loss, extra, outside);
+    p.stats[row] = make_float4(ref, loss == loss ? total : loss, TAIL ? mass : list_log, outside);
   }
 }
 
@@ -897,12 +1147,15 @@ vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
 // ---------------------------------------------------------------------------------------------
 // Launch
 // ---------------------------------------------------------------------------------------------
-// CTAs that share a row: one when the rows alone fill the machine, else as many (up to a portable
-// cluster) as still leave every thread a 16-byte load.
-int parts_for(int64_t rows, int vocab, int per_vector, int threads) {
+// CTAs that share a row: as many, up to `most`, as fit the machine at one CTA per SM and leave every
+// thread a 16-byte load. A second cluster on an SM costs more than it hides: 64 x 50304 bf16
+// log-probabilities take 7.3 us with two CTAs a row, 7.1 with four, 11.3 with eight; one row 6.3 with
+// eight against 7.8 with one. Joining top lists costs more with every CTA, hence `most` = 4 there: one
+// row with the 20 best 10.4 us with four, 10.5 with one, 12.5 with eight.
+int parts_for(int64_t rows, int vocab, int per_vector, int threads, int most) {
   const int vecs = vocab / per_vector;
   int parts = 1;
-  while (parts < kMaxCluster && rows * parts < 2 * device_sm_count() && vecs >= 2 * parts * threads)
+  while (parts < most && 2 * rows * parts <= device_sm_count() && vecs >= 2 * parts * threads)
     parts *= 2;
   return parts;
 }
@@ -929,7 +1182,7 @@ void launch_rows(Kernel kernel, int64_t ctas, int cluster, int threads, size_t s
 
 template <typename T, int THREADS>
 void logprobs_launch(const RowsView& view, TokenLogprobsArgs& a, int64_t rows, cudaStream_t stream) {
-  a.parts = parts_for(rows, a.vocab, Elem<T>::kN, THREADS);
+  a.parts = THREADS == 512 ? parts_for(rows, a.vocab, Elem<T>::kN, THREADS, a.top > 0 ? 4 : kMaxCluster) : 1;
   auto go = [&](auto kernel) {
     launch_rows(kernel, rows * a.parts, a.parts, THREADS, 0, view, a, stream);
   };
@@ -943,7 +1196,7 @@ void logprobs_launch(const RowsView& view, TokenLogprobsArgs& a, int64_t rows, c
 template <typename T, int THREADS>
 void distillation_launch(const RowsView& view, DistillationArgs& a, int64_t rows, cudaStream_t stream) {
   constexpr int N = Elem<T>::kN;
-  a.parts = parts_for(rows, a.vocab, N, THREADS);
+  a.parts = THREADS == 512 ? parts_for(rows, a.vocab, N, THREADS, kMaxCluster) : 1;
   if (!a.tail) {
     launch_rows(distillation_kernel<T, THREADS, false>, rows * a.parts, a.parts, THREADS, 0, view, a, stream);
     return;
@@ -968,8 +1221,42 @@ void grad_launch(const RowsView& view, VocabGradArgs& a, int64_t rows, bool dist
     launch_rows(vocab_grad_kernel<T, O, threads, false>, rows * a.parts, 1, threads, 0, view, a, stream);
 }
 
-// Rows of up to this many bytes get a small CTA: a large one would leave most of its threads idle.
-constexpr int64_t kSmallRowBytes = 16 * 1024;
+// Threads of a CTA, by what there is to hide. Measured on one B200 (50304 bf16 logits a row unless said
+// otherwise, log-probabilities / with the 20 best):
+//   many rows: small CTAs, of which many share an SM, so that one ends its row (two barriers and a
+//     chain of reductions) while others read: 8188 rows 124 / 179 us with 128 threads, 135 / 260 with
+//     256, 161 / 395 with 512. Rows of over 128 KB without a top list are long enough for 256: 4096 x
+//     131072 161 against 172 us.
+//   a few rows per SM: 700 rows 17.4 / 26.8 us with 256, 19.3 / 26.8 with 128.
+//   up to two rows per SM: 64 rows 7.3 / 10.5 us with 512, 10.5 / 14.5 with 256, 14.6 / 20.6 with 128;
+//     this is also the shape that cuts a row over a cluster.
+//   rows of up to 16 KB have too few vectors for more than 128 threads.
+//   a top list of more than 64 needs more than 128 lanes to take its bound from.
+int threads_for(int64_t rows, int64_t row_bytes, int top) {
+  const int sms = device_sm_count();
+  const bool small = row_bytes <= 16 * 1024;
+  if (rows <= 2 * sms && !small) return 512;
+  if (top > 64) return 256;
+  if (rows <= 6 * sms) return small ? 128 : 256;
+  return row_bytes <= 128 * 1024 || top > 0 ? 128 : 256;
+}
+
+template <typename T>
+void logprobs_by_shape(const RowsView& view, TokenLogprobsArgs& a, int64_t rows, cudaStream_t stream) {
+  switch (threads_for(rows, (int64_t)a.vocab * sizeof(T), a.top)) {
+    case 128: logprobs_launch<T, 128>(view, a, rows, stream); break;
+    case 256: logprobs_launch<T, 256>(view, a, rows, stream); break;
+    default: logprobs_launch<T, 512>(view, a, rows, stream); break;
+  }
+}
+template <typename T>
+void distillation_by_shape(const RowsView& view, DistillationArgs& a, int64_t rows, cudaStream_t stream) {
+  switch (threads_for(rows, (int64_t)a.vocab * sizeof(T), 0)) {
+    case 128: distillation_launch<T, 128>(view, a, rows, stream); break;
+    case 256: distillation_launch<T, 256>(view, a, rows, stream); break;
+    default: distillation_launch<T, 512>(view, a, rows, stream); break;
+  }
+}
 
 }  // namespace
 
@@ -978,20 +1265,10 @@ void token_logprobs(const RowsView& view, LogitType type, TokenLogprobsArgs args
   if (rows == 0) return;
   OB_CHECK(args.top >= 0 && args.top <= kMaxAlternatives && args.top <= args.vocab,
            "token_logprobs: bad number of alternatives");
-  const bool small = (int64_t)args.vocab * (type == LogitType::F32 ? 4 : 2) <= kSmallRowBytes;
   switch (type) {
-    case LogitType::F32:
-      small ? logprobs_launch<float, 128>(view, args, rows, stream)
-            : logprobs_launch<float, 512>(view, args, rows, stream);
-      break;
-    case LogitType::BF16:
-      small ? logprobs_launch<__nv_bfloat16, 128>(view, args, rows, stream)
-            : logprobs_launch<__nv_bfloat16, 512>(view, args, rows, stream);
-      break;
-    case LogitType::F16:
-      small ? logprobs_launch<__half, 128>(view, args, rows, stream)
-            : logprobs_launch<__half, 512>(view, args, rows, stream);
-      break;
+    case LogitType::F32: logprobs_by_shape<float>(view, args, rows, stream); break;
+    case LogitType::BF16: logprobs_by_shape<__nv_bfloat16>(view, args, rows, stream); break;
+    case LogitType::F16: logprobs_by_shape<__half>(view, args, rows, stream); break;
   }
 }
 
@@ -999,20 +1276,10 @@ void distillation_loss(const RowsView& view, LogitType type, DistillationArgs ar
                        cudaStream_t stream) {
   if (rows == 0) return;
   OB_CHECK(args.top >= 1 && args.top <= kMaxAlternatives, "distillation: bad length of the teacher's list");
-  const bool small = (int64_t)args.vocab * (type == LogitType::F32 ? 4 : 2) <= kSmallRowBytes;
   switch (type) {
-    case LogitType::F32:
-      small ? distillation_launch<float, 128>(view, args, rows, stream)
-            : distillation_launch<float, 512>(view, args, rows, stream);
-      break;
-    case LogitType::BF16:
-      small ? distillation_launch<__nv_bfloat16, 128>(view, args, rows, stream)
-            : distillation_launch<__nv_bfloat16, 512>(view, args, rows, stream);
-      break;
-    case LogitType::F16:
-      small ? distillation_launch<__half, 128>(view, args, rows, stream)
-            : distillation_launch<__half, 512>(view, args, rows, stream);
-      break;
+    case LogitType::F32: distillation_by_shape<float>(view, args, rows, stream); break;
+    case LogitType::BF16: distillation_by_shape<__nv_bfloat16>(view, args, rows, stream); break;
+    case LogitType::F16: distillation_by_shape<__half>(view, args, rows, stream); break;
   }
 }
 

@@ -411,11 +411,13 @@ def test_linear_form_over_several_chunks_and_fp32_masters(monkeypatch):
     whole, whole_grads = run()
     monkeypatch.setattr(logprobs, "_chunk_rows", lambda tokens, vocab: 128)
     parts, part_grads = run()
-    assert torch.equal(whole.logprobs, parts.logprobs) and torch.equal(whole.top_tokens, parts.top_tokens)
+    # how a row is cut over threads depends on the number of rows: each side is off by a slack
+    assert torch.equal(whole.top_tokens, parts.top_tokens)
+    torch.testing.assert_close(parts.logprobs, whole.logprobs, rtol=16 * 2.0**-24,
+                               atol=4 * _slack(777))
     assert whole_grads[0].dtype == torch.float32 and whole_grads[1].dtype == torch.float32
-    torch.testing.assert_close(part_grads[0], whole_grads[0], rtol=0, atol=0)
-    # the weight gradient adds fp32 sums of six chunks in place of one sum
-    torch.testing.assert_close(part_grads[1], whole_grads[1], rtol=1e-5, atol=1e-4)
+    for a, b in zip(part_grads, whole_grads):  # bf16 roundings of the logits' gradient may differ
+        assert (a - b).norm() / b.norm() < 2 * 2.0**-9
 
 
 # -- how they are called ---------------------------------------------------------------------------------
