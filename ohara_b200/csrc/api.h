@@ -283,4 +283,30 @@ struct VocabGradArgs {
 void vocab_grad(const RowsView& view, LogitType type, LogitType out_type, VocabGradArgs args,
                 int64_t rows, bool distill, cudaStream_t stream);
 
+// vocab_gemm_sm100.cu: the same two operators from bf16 hidden states (M x K) and projection (N x K),
+// without logits in memory. `partial` has linear_head_halves(N) x linear_head_rows(M) elements,
+// `picked` one float per named token, `marks` M x linear_head_mark_words(N) words (with `tail`). The
+// top list of TokenLogprobsArgs is not supported here.
+struct LinearHead {
+  const void* hidden;
+  const void* weight;
+  int64_t ldh, ldw;  // row pitches in elements, multiples of 8; 16-byte aligned bases
+  int M, N, K;       // K a multiple of 8
+};
+int64_t linear_head_halves(int vocab);
+int64_t linear_head_rows(int64_t rows);
+int64_t linear_head_mark_words(int vocab);
+void linear_token_logprobs(const LinearHead& head, const TokenLogprobsArgs& args, float4* partial,
+                           float* picked, cudaStream_t stream);
+void linear_distillation(const LinearHead& head, const DistillationArgs& args, float4* partial,
+                         float* picked, uint32_t* marks, cudaStream_t stream);
+// d(loss) / d(logits) in bf16 into args.out (pitch a multiple of 8, 16-byte aligned); `picked` from the
+// forward pass, `coef` M elements of scratch. grad_top is not supported here.
+void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool distill,
+                       const float* picked, float4* coef, cudaStream_t stream);
+
+// out (bf16 or fp32) = parts[0] + parts[1] + ... of a product whose reduction was cut in `count` pieces.
+void sum_parts(const float* parts, void* out, bool out_f32, int64_t elements, int count,
+               cudaStream_t stream);
+
 }  // namespace ob

@@ -13,6 +13,9 @@ std::vector<torch::Tensor> pscan_cpu_bwd(const torch::Tensor& a, const torch::Te
                                          const torch::Tensor& dh);
 }  // namespace ob_cpu
 
+// vocab_ops.cpp: log-probabilities and distillation over the vocabulary, with their autograd nodes
+void register_vocab_ops(pybind11::module_& m);
+
 namespace {
 
 using torch::Tensor;
@@ -311,197 +314,6 @@ std::vector<Tensor> cross_entropy_rows(Tensor& logits, const Tensor& targets,
                          logits.stride(0), ignore_index, write_grad, current_stream());
   if (want_correct) return {loss, lse, correct};
   return {loss, lse};
-}
-
-// -- rows of logits over the vocabulary (vocab_rows.cu) ---------------------------------------------
-ob::LogitType logit_type(const Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
-    case torch::kFloat32: return ob::LogitType::F32;
-    case torch::kBFloat16: return ob::LogitType::BF16;
-    case torch::kFloat16: return ob::LogitType::F16;
-    default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16");
-  }
-}
-
-// Any strides over the leading dimensions that two of them can express (slices of a padded vocabulary,
-// `logits[:, :-1]`, expanded batches); false where the rows have to be copied together first.
-bool rows_view(const Tensor& t, ob::RowsView& view) {
-  const int64_t vocab = t.size(-1);
-  if (vocab > 1 && t.stride(-1) != 1) return false;
-  int64_t sizes[2] = {1, 1}, strides[2] = {0, 0};  // innermost first
-  int used = 0;
-  for (int64_t d = t.dim() - 2; d >= 0; --d) {
-    const int64_t n = t.size(d), st = t.stride(d);
-    if (n == 1) continue;
-    if (used > 0 && st == strides[used - 1] * sizes[used - 1]) {
-      sizes[used - 1] *= n;
-    } else if (used < 2) {
-      sizes[used] = n;
-      strides[used] = st;
-      ++used;
-    } else {
-      return false;
-    }
-  }
-  view.base = t.data_ptr();
-  view.inner = sizes[0];
-  view.inner_stride = strides[0];
-  view.outer_stride = strides[1];
-  return true;
-}
-
-struct LogitRows {
-  Tensor t;  // keeps a copy alive
-  ob::RowsView view;
-  ob::LogitType type;
-  int64_t rows;
-  int vocab;
-};
-LogitRows logit_rows(const Tensor& logits) {
-  check_cuda(logits, "logits");
-  TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "logits need a vocabulary dimension");
-  TORCH_CHECK(logits.size(-1) < (1ll << 31) - 1024, "vocabulary too large");
-  LogitRows r;
-  r.t = logits;
-  r.type = logit_type(logits, "logits");
-  if (!rows_view(r.t, r.view)) {
-    r.t = logits.contiguous();
-    TORCH_CHECK(rows_view(r.t, r.view));
-  }
-  r.vocab = (int)logits.size(-1);
-  r.rows = logits.numel() / r.vocab;
-  return r;
-}
-
-// A contiguous per-row operand of `numel` elements on the logits' device.
-template <typename S>
-S* row_operand(const c10::optional<Tensor>& t, const Tensor& logits, torch::ScalarType type,
-               int64_t numel, const char* name) {
-  if (!t.has_value()) return nullptr;
-  TORCH_CHECK(t->device() == logits.device(), name, " must be on the logits' device");
-  TORCH_CHECK(t->scalar_type() == type && t->is_contiguous() && t->numel() == numel, name,
-              " must be a contiguous tensor of ", numel, " elements of type ", c10::toString(type));
-  return t->data_ptr<S>();
-}
-
-// Writes into the given outputs (logprobs / entropy / top lists may be absent).
-void token_logprobs_fwd(const Tensor& logits, const c10::optional<Tensor>& tokens,
-                        double inv_temperature, int64_t top, int64_t ignore_index,
-                        const c10::optional<Tensor>& logprobs, const c10::optional<Tensor>& entropy,
-                        const c10::optional<Tensor>& top_logprobs,
-                        const c10::optional<Tensor>& top_tokens, const Tensor& stats) {
-  const c10::cuda::CUDAGuard guard(logits.device());
-  const LogitRows r = logit_rows(logits);
-  TORCH_CHECK(top >= 0 && top <= ob::kMaxAlternatives && top <= r.vocab, "bad number of alternatives");
-  TORCH_CHECK((top > 0) == top_logprobs.has_value() && (top > 0) == top_tokens.has_value(),
-              "top lists and their length do not match");
-  TORCH_CHECK(tokens.has_value() || !logprobs.has_value(), "log-probabilities need tokens");
-  ob::TokenLogprobsArgs a = {};
-  a.tokens = row_operand<int64_t>(tokens, logits, torch::kInt64, r.rows, "tokens");
-  a.logprobs = row_operand<float>(logprobs, logits, torch::kFloat32, r.rows, "logprobs");
-  a.entropy = row_operand<float>(entropy, logits, torch::kFloat32, r.rows, "entropy");
-  a.top_logprobs = row_operand<float>(top_logprobs, logits, torch::kFloat32, r.rows * top, "top_logprobs");
-  a.top_tokens = row_operand<int64_t>(top_tokens, logits, torch::kInt64, r.rows * top, "top_tokens");
-  a.stats = reinterpret_cast<float4*>(
-      row_operand<float>(stats, logits, torch::kFloat32, r.rows * 4, "stats"));
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(a.stats) % 16 == 0, "stats must be 16-byte aligned");
-  a.ignore_index = ignore_index;
-  a.inv_temperature = (float)inv_temperature;
-  a.vocab = r.vocab;
-  a.top = (int)top;
-  ob::token_logprobs(r.view, r.type, a, r.rows, current_stream());
-}
-
-void distillation_fwd(const Tensor& logits, const Tensor& teacher, const Tensor& tokens,
-                      double inv_temperature, bool tail, const Tensor& loss, const Tensor& stats) {
-  const c10::cuda::CUDAGuard guard(logits.device());
-  const LogitRows r = logit_rows(logits);
-  const int64_t top = tokens.size(-1);
-  TORCH_CHECK(top >= 1 && top <= ob::kMaxAlternatives, "bad length of the teacher's list");
-  ob::DistillationArgs a = {};
-  a.teacher = row_operand<float>(teacher, logits, torch::kFloat32, r.rows * top, "teacher_logprobs");
-  a.tokens = row_operand<int64_t>(tokens, logits, torch::kInt64, r.rows * top, "teacher_tokens");
-  a.loss = row_operand<float>(loss, logits, torch::kFloat32, r.rows, "loss");
-  a.stats = reinterpret_cast<float4*>(
-      row_operand<float>(stats, logits, torch::kFloat32, r.rows * 4, "stats"));
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(a.stats) % 16 == 0, "stats must be 16-byte aligned");
-  a.inv_temperature = (float)inv_temperature;
-  a.vocab = r.vocab;
-  a.top = (int)top;
-  a.tail = tail ? 1 : 0;
-  ob::distillation_loss(r.view, r.type, a, r.rows, current_stream());
-}
-
-// Where the gradient goes: `out` (2-D, row pitch free), or a new tensor of the logits' shape and type.
-Tensor grad_target(const Tensor& logits, const LogitRows& r, const c10::optional<Tensor>& out,
-                   ob::VocabGradArgs& a, ob::LogitType& type) {
-  Tensor o = out.has_value() ? *out : torch::empty(logits.sizes(), logits.options());
-  TORCH_CHECK(o.device() == logits.device(), "out must be on the logits' device");
-  type = logit_type(o, "out");
-  a.out = o.data_ptr();
-  a.out_pitch = r.vocab;
-  if (out.has_value()) {
-    TORCH_CHECK(o.dim() == 2 && o.size(0) == r.rows && o.size(1) == r.vocab && o.stride(1) == 1 &&
-                    (r.rows <= 1 || o.stride(0) >= r.vocab),
-                "out must have a row for each row of the logits");
-    a.out_pitch = o.stride(0);
-  }
-  return o;
-}
-
-Tensor token_logprobs_bwd(const Tensor& logits, const Tensor& stats, const c10::optional<Tensor>& tokens,
-                          const c10::optional<Tensor>& top_tokens,
-                          const c10::optional<Tensor>& grad, const c10::optional<Tensor>& grad_entropy,
-                          const c10::optional<Tensor>& grad_top, double inv_temperature,
-                          const c10::optional<Tensor>& out) {
-  const c10::cuda::CUDAGuard guard(logits.device());
-  const LogitRows r = logit_rows(logits);
-  ob::VocabGradArgs a = {};
-  ob::LogitType out_type;
-  Tensor o = grad_target(logits, r, out, a, out_type);
-  const int64_t top = grad_top.has_value() ? grad_top->size(-1) : 0;
-  TORCH_CHECK(top <= ob::kMaxAlternatives, "bad number of alternatives");
-  TORCH_CHECK(!grad.has_value() || tokens.has_value(), "a log-probability gradient needs tokens");
-  TORCH_CHECK(!grad_top.has_value() || top_tokens.has_value(), "a top-list gradient needs its tokens");
-  a.stats = reinterpret_cast<const float4*>(
-      row_operand<float>(stats, logits, torch::kFloat32, r.rows * 4, "stats"));
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(a.stats) % 16 == 0, "stats must be 16-byte aligned");
-  a.tokens = row_operand<int64_t>(tokens, logits, torch::kInt64, r.rows, "tokens");
-  a.grad = row_operand<float>(grad, logits, torch::kFloat32, r.rows, "grad");
-  a.grad_entropy = row_operand<float>(grad_entropy, logits, torch::kFloat32, r.rows, "grad_entropy");
-  if (top > 0) {
-    a.grad_top = row_operand<float>(grad_top, logits, torch::kFloat32, r.rows * top, "grad_top");
-    a.top_tokens = row_operand<int64_t>(top_tokens, logits, torch::kInt64, r.rows * top, "top_tokens");
-  }
-  a.inv_temperature = (float)inv_temperature;
-  a.vocab = r.vocab;
-  a.top = (int)top;
-  ob::vocab_grad(r.view, r.type, out_type, a, r.rows, false, current_stream());
-  return o;
-}
-
-Tensor distillation_bwd(const Tensor& logits, const Tensor& stats, const Tensor& teacher,
-                        const Tensor& tokens, const Tensor& grad, double inv_temperature, bool tail,
-                        const c10::optional<Tensor>& out) {
-  const c10::cuda::CUDAGuard guard(logits.device());
-  const LogitRows r = logit_rows(logits);
-  ob::VocabGradArgs a = {};
-  ob::LogitType out_type;
-  Tensor o = grad_target(logits, r, out, a, out_type);
-  const int64_t top = tokens.size(-1);
-  TORCH_CHECK(top >= 1 && top <= ob::kMaxAlternatives, "bad length of the teacher's list");
-  a.stats = reinterpret_cast<const float4*>(
-      row_operand<float>(stats, logits, torch::kFloat32, r.rows * 4, "stats"));
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(a.stats) % 16 == 0, "stats must be 16-byte aligned");
-  a.grad = row_operand<float>(grad, logits, torch::kFloat32, r.rows, "grad");
-  a.teacher = row_operand<float>(teacher, logits, torch::kFloat32, r.rows * top, "teacher_logprobs");
-  a.tokens = row_operand<int64_t>(tokens, logits, torch::kInt64, r.rows * top, "teacher_tokens");
-  a.inv_temperature = (float)inv_temperature;
-  a.vocab = r.vocab;
-  a.top = (int)top;
-  a.tail = tail ? 1 : 0;
-  ob::vocab_grad(r.view, r.type, out_type, a, r.rows, true, current_stream());
-  return o;
 }
 
 void scale_by_scalar(Tensor& x, const Tensor& scalar) {
@@ -1397,15 +1209,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_step", &adamw_step);
   m.def("cross_entropy_rows", &cross_entropy_rows);
   m.def("scale_by_scalar", &scale_by_scalar);
-  m.attr("MAX_ALTERNATIVES") = ob::kMaxAlternatives;
-  m.def("token_logprobs_fwd", &token_logprobs_fwd);
-  m.def("token_logprobs_bwd", &token_logprobs_bwd, py::arg("logits"), py::arg("stats"),
-        py::arg("tokens"), py::arg("top_tokens"), py::arg("grad"), py::arg("grad_entropy"),
-        py::arg("grad_top"), py::arg("inv_temperature"), py::arg("out") = py::none());
-  m.def("distillation_fwd", &distillation_fwd);
-  m.def("distillation_bwd", &distillation_bwd, py::arg("logits"), py::arg("stats"),
-        py::arg("teacher"), py::arg("tokens"), py::arg("grad"), py::arg("inv_temperature"),
-        py::arg("tail"), py::arg("out") = py::none());
+  register_vocab_ops(m);
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("muon_prepare", &muon_prepare);
   m.def("muon_variance", &muon_variance);

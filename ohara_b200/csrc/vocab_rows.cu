@@ -26,16 +26,14 @@
 #include "api.h"
 #include "common.cuh"
 #include "host_utils.h"
+#include "vocab_rows.cuh"
 
 namespace ob {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-// A teacher's mass outside its list of up to this much is the rounding of the list's sum (K terms of
-// relative error 2^-24 and the teacher's own) and counts as none: the student may have no token there.
-constexpr float kLeastRest = 1e-6f;
+using namespace vocab;
+
 constexpr int kUnroll = 4;       // 16-byte loads in flight per thread
 constexpr int kMaxCluster = 8;   // the portable cluster size
 
@@ -43,33 +41,6 @@ constexpr int kMaxCluster = 8;   // the portable cluster size
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// Two floats in one register pair: sm_100 adds, multiplies and fuses them with one instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 both(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 
@@ -171,38 +142,8 @@ __device__ __forceinline__ uint32_t code_index(uint64_t code) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Running statistics of the softmax of scaled logits (c = log2(e) / T): `m` the maximum seen (-inf:
-// nothing finite yet), `s` the sum of e = 2^((x - m) c), and `w` by kind
-//   kSum      nothing
-//   kEntropy  the sum of e (x - m)
-//   kSplit    the sum of e over the tokens outside the teacher's list; `s` is the sum inside it
+// A thread's part of a row
 // ---------------------------------------------------------------------------------------------
-enum Kind { kSum, kEntropy, kSplit };
-
-struct Stats {
-  float m, s, w;
-};
-
-__device__ __forceinline__ float reference_of(float m) { return m == -INFINITY ? 0.f : m; }
-
-// Moves the sums from maximum `a.m` to `m` (>= a.m).
-template <Kind K>
-__device__ __forceinline__ void rebase(Stats& a, float m, float c) {
-  if (m == a.m) return;
-  const float shift = a.m - m;  // < 0; -inf while nothing was seen or where the gap overflows
-  const float f = fast_exp2(shift * c);
-  if (f == 0.f) {
-    // an empty or vanished sum becomes zero (0 * inf below would not), a NaN stays
-    a.s = a.s == a.s ? 0.f : a.s;
-    if (K != kSum) a.w = a.w == a.w ? 0.f : a.w;
-  } else {
-    if (K == kEntropy) a.w = f * fmaf(a.s, shift, a.w);
-    if (K == kSplit) a.w *= f;
-    a.s *= f;
-  }
-  a.m = m;
-}
-
 // A thread's sums over the logits it has read, even and odd elements apart.
 struct Running {
   float m;
@@ -270,26 +211,6 @@ __device__ __forceinline__ Running first_of(float x, float c, bool in_list) {
 __device__ __forceinline__ Stats folded(const Running& a) {
   const float2 s = both(a.s), w = both(a.w);
   return Stats{a.m, s.x + s.y, w.x + w.y};
-}
-
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// One maximum for the warp first, so that every lane moves its sums once.
-template <Kind K>
-__device__ __forceinline__ Stats warp_merge(Stats a, float c) {
-  rebase<K>(a, warp_max(a.m), c);
-  a.s = warp_sum(a.s);
-  if (K != kSum) a.w = warp_sum(a.w);
-  return a;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -839,9 +760,6 @@ __device__ __forceinline__ float block_sum(float v, float* scratch, int warps) {
   for (int i = 0; i < warps; ++i) total += scratch[i];
   return total;
 }
-// A lane's share of the teacher's list: entries lane, lane + 32, ...
-constexpr int kEntriesPerLane = kMaxAlternatives / 32;
-
 // One bit per logit of the slice marks the listed tokens, a byte per 16-byte vector, so that the sum
 // over the others is formed without a subtraction (1 - sum of the listed q would cancel away exactly
 // where the student agrees with the teacher).
@@ -866,14 +784,8 @@ distillation_kernel(const RowsView view, const DistillationArgs p) {
   const int64_t* tokens = p.tokens + row * p.top;
   const float* teacher = p.teacher + row * p.top;
 
-  // ---- does the list teach anything? (every warp looks for itself) ------------------------------
-  bool counts = false;
-  for (int k = lane; k < p.top; k += 32) counts |= tokens[k] >= 0 && (TAIL || teacher[k] != -INFINITY);
-  if (!__any_sync(0xffffffffu, counts)) {  // an empty list: the row is not read
-    if (part == 0 && tid == 0) {
-      p.loss[row] = 0.f;
-      p.stats[row] = make_float4(0.f, INFINITY, 0.f, 0.f);
-    }
+  if (!list_counts(p, row)) {  // every warp looks for itself; the row is not read
+    if (part == 0 && tid == 0) skip_row(p, row);
     return;
   }
   if (parts > 1) cluster_arrive();
@@ -962,56 +874,24 @@ distillation_kernel(const RowsView view, const DistillationArgs p) {
   }
   if (part != 0 || warp != 0) return;
 
-  // ---- the row's loss, by one warp ---------------------------------------------------------------
-  const float ref = reference_of(all.m), outside = all.w;
-  const float total = TAIL ? all.s + outside : all.s;
-  const float log_s = logf(total);
-  float list_log = 0.f;  // log-sum of the list, which renormalises it
-  if (!TAIL) {
-    float high = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kEntriesPerLane; ++i) high = fmaxf(high, value[i]);
-    high = warp_max(high);
-    float mass = 0.f;
-#pragma unroll
-    for (int i = 0; i < kEntriesPerLane; ++i) mass += expf(value[i] - high);
-    list_log = high + logf(warp_sum(mass));
-  }
-  float loss = 0.f, mass = 0.f;
-#pragma unroll
-  for (int i = 0; i < kEntriesPerLane; ++i) {
-    const float log_p = value[i] - list_log;
-    const float weight = expf(log_p);
-    mass += weight;
-    if (weight != 0.f) loss += weight * (log_p - fmaf(picked[i] - ref, p.inv_temperature, -log_s));
-  }
-  loss = warp_sum(loss);
-  mass = warp_sum(mass);
-  if (TAIL) {
-    const float rest = 1.f - mass;
-    if (!(rest <= kLeastRest)) loss += rest * (logf(rest) - (logf(outside) - log_s));
-  }
-  if (lane == 0) {
-    p.loss[row] = loss;
-    // a NaN loss has a NaN gradient, also where it comes from a token outside the vocabulary
-    p.stats[row] = make_float4(ref, loss == loss ? total : loss, TAIL ? mass : list_log, outside);
-  }
+  finish_distillation<TAIL>(p, row, value, picked, reference_of(all.m), TAIL ? all.s + all.w : all.s,
+                            all.w);
 }
 
 // ---------------------------------------------------------------------------------------------
 // Gradients
 // ---------------------------------------------------------------------------------------------
-// Both operators' gradients are  e (slope t + level)  with t = (x - m) c and e = 2^t for the tokens
-// that no entry names, so one streaming pass writes that everywhere and, after a barrier, one thread
-// per named token overwrites its element with the full sum (rounded once; a token that several entries
-// name is written by the first of them with all their weights, so the order of nothing matters).
+// One streaming pass writes the gradient of an unnamed token everywhere (see `GradRow`) and, after a
+// barrier, one thread per named token overwrites its element with the full sum (rounded once; a token
+// that several entries name is written by the first of them with all their weights, so the order of
+// nothing matters).
 template <typename T, typename O, int THREADS, bool DISTILL>
 __global__ void __launch_bounds__(THREADS)
 vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
   constexpr int N = Elem<T>::kN;
   __shared__ float reduce[THREADS / 32];
   __shared__ int64_t entry_token[kMaxAlternatives + 1];
-  __shared__ float entry_weight[kMaxAlternatives + 1];
+  __shared__ float entry_weights[kMaxAlternatives + 1];
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / p.parts;
   const int part = (int)(blockIdx.x - row * p.parts);
@@ -1021,76 +901,42 @@ vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
   O* out = static_cast<O*>(p.out) + row * p.out_pitch;
   const Slice sl = slice_of(x, vocab, part, p.parts);
   const int edge = edge_index(sl, vocab, part);
-  const float4 st = p.stats[row];
-  const float ref = st.x, total = st.y;
 
-  // ---- the row's coefficients ------------------------------------------------------------------
-  float slope = 0.f, level, level_named;  // `level_named`: for the tokens that an entry names
-  int entries = 0;
-  bool zero = total == INFINITY;  // the forward pass skipped this row
-  if (!zero) {
-    if constexpr (DISTILL) {
-      const float g = p.grad[row] * p.inv_temperature;
-      zero = g == 0.f;
-      entries = p.top;
-      float mass = 1.f, rest = 0.f;
-      if (p.tail) {
-        mass = st.z;
-        rest = 1.f - mass <= kLeastRest ? 0.f : 1.f - mass;
-        mass += rest;
+  // ---- the row's coefficients and entries --------------------------------------------------------
+  int entries = DISTILL ? p.top : 1;
+  float g_top = 0.f;
+  bool any_top = false;
+  if constexpr (DISTILL) {
+    if (tid < entries) {
+      entry_token[tid] = p.tokens[row * p.top + tid];
+      entry_weights[tid] = entry_token[tid] < 0 ? 0.f : entry_weight<true>(p, row, tid);
+    }
+  } else {
+    if (tid == 0) {
+      entry_token[0] = p.grad != nullptr ? p.tokens[row] : -1;
+      entry_weights[0] = entry_weight<false>(p, row, 0);
+    }
+    if (p.grad_top != nullptr) {
+      entries += p.top;
+      float mine = 0.f;
+      if (tid < p.top) {
+        mine = p.grad_top[row * p.top + tid];
+        entry_token[1 + tid] = p.top_tokens[row * p.top + tid];
+        entry_weights[1 + tid] = mine * p.inv_temperature;
       }
-      level_named = g * mass / total;
-      // without outside mass every unnamed token has e = 0
-      level = (rest > 0.f && st.w > 0.f) ? g * (mass / total - rest / st.w) : level_named;
-      if (!zero && tid < entries) {
-        const int64_t token = p.tokens[row * p.top + tid];
-        const float value = p.teacher[row * p.top + tid];
-        entry_token[tid] = token;
-        entry_weight[tid] = token < 0 ? 0.f : -g * expf(p.tail ? value : value - st.z);
-      }
-    } else {
-      float g = 0.f, gh = 0.f, g_top = 0.f, any = 0.f;
-      int64_t token = -1;
-      if (p.grad != nullptr) {
-        g = p.grad[row];
-        token = p.tokens[row];
-        if (g != 0.f && (token < 0 || token >= vocab)) g = __uint_as_float(0x7fffffffu);
-      }
-      if (p.grad_entropy != nullptr) gh = p.grad_entropy[row];
-      entries = 1;
-      if (p.grad_top != nullptr) {
-        entries += p.top;
-        float mine = 0.f;
-        if (tid < p.top) {
-          mine = p.grad_top[row * p.top + tid];
-          entry_token[1 + tid] = p.top_tokens[row * p.top + tid];
-          entry_weight[1 + tid] = mine * p.inv_temperature;
-        }
-        g_top = block_sum(mine, reduce, THREADS / 32);
-        any = __syncthreads_or(mine != 0.f) ? 1.f : 0.f;
-      }
-      zero = g == 0.f && gh == 0.f && any == 0.f;
-      if (tid == 0) {
-        entry_token[0] = token;
-        entry_weight[0] = g * p.inv_temperature;
-      }
-      const float inv = p.inv_temperature / total;
-      level = level_named = -inv * (g + g_top + gh * (st.z - logf(total)));
-      slope = -inv * gh * kLn2;
+      g_top = block_sum(mine, reduce, THREADS / 32);
+      any_top = __syncthreads_or(mine != 0.f) != 0;
     }
   }
-  if (zero) {  // also where the logits hold NaN: nothing of this row was asked for
-    entries = 0;
-    slope = level = 0.f;
-  }
+  const GradRow g = grad_row<DISTILL>(p, row, g_top, any_top);
+  const bool zero = g.zero;
 
   // ---- every token -----------------------------------------------------------------------------
-  auto value = [&](float f, float lv) {
-    // e is 0 from t = -150 down; the clamp keeps `slope t` finite there (masked logits: t = -inf)
-    const float t = fmaxf((f - ref) * c, -1.0e4f);
-    return fast_exp2(t) * fmaf(slope, t, lv);
+  auto value = [&](float f, float level) {
+    const float t = grad_exponent(f, g.ref, c);
+    return fast_exp2(t) * fmaf(g.slope, t, level);
   };
-  if (edge >= 0) Elem<O>::store(out + edge, zero ? 0.f : value(Elem<T>::load(x + edge), level));
+  if (edge >= 0) Elem<O>::store(out + edge, zero ? 0.f : value(Elem<T>::load(x + edge), g.level));
   const uint4* body = reinterpret_cast<const uint4*>(x + sl.head);
   O* out_body = out + sl.head;
   const bool aligned = reinterpret_cast<uintptr_t>(out_body) % (N * sizeof(O)) == 0;
@@ -1110,7 +956,7 @@ vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
       } else {
         Elem<T>::unpack(raw[u], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = value(f[i], level);
+        for (int i = 0; i < N; ++i) f[i] = value(f[i], g.level);
       }
       if (aligned) {
         store_vec(out_body + (int64_t)v * N, f);
@@ -1120,7 +966,7 @@ vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
       }
     }
   }
-  if (entries == 0) return;
+  if (zero) return;
 
   // ---- the named tokens of this part -----------------------------------------------------------
   __syncthreads();
@@ -1136,10 +982,10 @@ vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
     }
     for (int j = 0; mine && j < tid; ++j) mine = entry_token[j] != token;
     if (mine) {
-      float weight = entry_weight[tid];
+      float weight = entry_weights[tid];
       for (int j = tid + 1; j < entries; ++j)
-        if (entry_token[j] == token) weight += entry_weight[j];
-      Elem<O>::store(out + token, value(Elem<T>::load(x + token), level_named) + weight);
+        if (entry_token[j] == token) weight += entry_weights[j];
+      Elem<O>::store(out + token, value(Elem<T>::load(x + token), g.level_named) + weight);
     }
   }
 }

@@ -21,7 +21,6 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from ._ext import ext
 
@@ -165,52 +164,16 @@ def _check_logits(logits: Tensor) -> None:
         raise TypeError(f"logits must be floating point, got {logits.dtype}")
 
 
-def _as_tokens(tokens: Tensor) -> Tensor:
-    return (tokens if tokens.dtype == torch.int64 else tokens.long()).contiguous()
-
-
-def _as_f32(t: Tensor | None) -> Tensor | None:
-    return None if t is None else (t if t.dtype == torch.float32 else t.float()).contiguous()
+def _results(found: list, tokens: Tensor | None, entropy: bool, top: int) -> TokenLogprobs:
+    """The extension returns what was asked for, in order."""
+    each = iter(found)
+    return TokenLogprobs(None if tokens is None else next(each), next(each) if entropy else None,
+                         next(each) if top else None, next(each) if top else None)
 
 
 # --------------------------------------------------------------------------------------------------
 # On given logits
 # --------------------------------------------------------------------------------------------------
-def _empty_results(lead, device, tokens, entropy: bool, top: int):
-    f32 = dict(device=device, dtype=torch.float32)
-    rows = math.prod(lead)
-    return (torch.empty(lead, **f32) if tokens is not None else None,
-            torch.empty(lead, **f32) if entropy else None,
-            torch.empty((*lead, top), **f32) if top else None,
-            torch.empty((*lead, top), device=device, dtype=torch.int64) if top else None,
-            torch.empty((rows, 4), **f32))
-
-
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits: Tensor, tokens: Tensor | None, inv_temperature: float, entropy: bool,
-                top: int, ignore_index: int):
-        out = _empty_results(logits.shape[:-1], logits.device, tokens, entropy, top)
-        logprobs, h, top_logprobs, top_tokens, stats = out
-        ext().token_logprobs_fwd(logits, tokens, inv_temperature, top, ignore_index, *out)
-        ctx.set_materialize_grads(False)
-        if top:
-            ctx.mark_non_differentiable(top_tokens)
-        ctx.save_for_backward(logits, tokens, top_tokens, stats)
-        ctx.inv_temperature = inv_temperature
-        return logprobs, h, top_logprobs, top_tokens
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_logprobs, d_entropy, d_top, _):
-        logits, tokens, top_tokens, stats = ctx.saved_tensors
-        if d_logprobs is None and d_entropy is None and d_top is None:
-            return (None,) * 6
-        d = ext().token_logprobs_bwd(logits, stats, tokens, top_tokens, _as_f32(d_logprobs),
-                                     _as_f32(d_entropy), _as_f32(d_top), ctx.inv_temperature)
-        return (d, None, None, None, None, None)
-
-
 def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, temperature: float = 1.0,
                    entropy: bool = False, top: int = 0,
                    ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
@@ -230,30 +193,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, *, temperature:
     if not logits.is_cuda:
         return token_logprobs_reference(logits, tokens, temperature=temperature, entropy=entropy,
                                         top=top, ignore_index=ignore_index)
-    tokens = None if tokens is None else _as_tokens(tokens)
-    return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, 1.0 / temperature, bool(entropy),
-                                                 int(top), int(ignore_index)))
-
-
-class _DistillationFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits: Tensor, teacher: Tensor, tokens: Tensor, inv_temperature: float,
-                tail: bool):
-        loss = torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32)
-        stats = torch.empty((loss.numel(), 4), device=logits.device, dtype=torch.float32)
-        ext().distillation_fwd(logits, teacher, tokens, inv_temperature, tail, loss, stats)
-        ctx.save_for_backward(logits, teacher, tokens, stats)
-        ctx.inv_temperature = inv_temperature
-        ctx.tail = tail
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss: Tensor):
-        logits, teacher, tokens, stats = ctx.saved_tensors
-        d = ext().distillation_bwd(logits, stats, teacher, tokens, _as_f32(d_loss),
-                                   ctx.inv_temperature, ctx.tail)
-        return d, None, None, None, None
+    found = ext().token_logprobs(logits, tokens, 1.0 / temperature, bool(entropy), top, ignore_index)
+    return _results(found, tokens, entropy, top)
 
 
 def distillation_loss(logits: Tensor, teacher_logprobs: Tensor, teacher_tokens: Tensor, *,
@@ -279,147 +220,17 @@ def distillation_loss(logits: Tensor, teacher_logprobs: Tensor, teacher_tokens: 
     if not logits.is_cuda:
         return distillation_loss_reference(logits, teacher_logprobs, teacher_tokens,
                                            temperature=temperature, tail=tail)
-    return _DistillationFn.apply(logits, _as_f32(teacher_logprobs), _as_tokens(teacher_tokens),
-                                 1.0 / temperature, bool(tail))
+    return ext().distillation_loss(logits, teacher_logprobs, teacher_tokens, 1.0 / temperature,
+                                   bool(tail))
 
 
 # --------------------------------------------------------------------------------------------------
 # From hidden states
 # --------------------------------------------------------------------------------------------------
-def _chunk_rows(tokens: int, vocab: int) -> int:
-    budget = 1024 * 1024 * 1024 // (4 * max(vocab, 1))
-    rows = max(128, (budget // 128) * 128)
-    return min(rows, max(128, ((tokens + 127) // 128) * 128))
-
-
-class _HeadChunks:
-    """The logits of ``hidden @ weight.T`` chunk by chunk: fp32, because the log-probabilities of a
-    bf16 logit of size 10 would be off by 0.03, in one buffer of a gigabyte that every chunk reuses."""
-
-    def __init__(self, hidden: Tensor, weight: Tensor):
-        from . import bf16_weight
-
-        h2 = hidden.reshape(-1, hidden.shape[-1])
-        self.h2 = (h2 if h2.dtype == torch.bfloat16 else h2.to(torch.bfloat16)).contiguous()
-        self.w16 = bf16_weight(weight)
-        self.tokens, self.vocab = self.h2.shape[0], weight.shape[0]
-        self.rows = _chunk_rows(self.tokens, self.vocab)
-        self.pitch = (self.vocab + 7) // 8 * 8
-        n = min(self.rows, max(self.tokens, 1))
-        self.buffer = torch.empty(n, self.pitch, device=self.h2.device, dtype=torch.float32)
-
-    def __iter__(self):
-        from . import matmul_nt
-
-        for start in range(0, self.tokens, self.rows):
-            stop = min(start + self.rows, self.tokens)
-            logits = self.buffer[:stop - start, :self.vocab]
-            matmul_nt(self.h2[start:stop], self.w16, out=logits)
-            yield slice(start, stop), logits
-
-
-def _head_backward(ctx, hidden: Tensor, weight: Tensor, gradient_of):
-    """Gradients of ``hidden`` and ``weight`` from ``gradient_of(rows, logits, out)``, which writes
-    d(loss) / d(logits) of a chunk. The chunk's gradient is rounded to bf16, the operand type of the
-    two products; both accumulate in fp32, the weight's over all chunks."""
-    from . import matmul_nn
-
-    chunks = _HeadChunks(hidden, weight)
-    need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    device = chunks.h2.device
-    dh = torch.empty_like(chunks.h2) if need_dh else None
-    dw = torch.zeros(weight.shape, device=device, dtype=torch.float32) if need_dw else None
-    grads = torch.empty(chunks.buffer.shape, device=device, dtype=torch.bfloat16)
-    for rows, logits in chunks:
-        d = grads[:logits.shape[0], :chunks.vocab]
-        gradient_of(rows, logits, d)
-        if need_dh:
-            matmul_nn(d, chunks.w16, out=dh[rows])
-        if need_dw:
-            # one split of the token dimension: the order of the sum is fixed
-            ext().gemm(d, chunks.h2[rows], dw, chunks.vocab, dw.shape[1], d.shape[0], True, True, 1,
-                       True, 1.0, None, None)
-    if need_dh:
-        dh = dh.view(hidden.shape)
-        dh = dh if dh.dtype == hidden.dtype else dh.to(hidden.dtype)
-    if need_dw and dw.dtype != weight.dtype:
-        dw = dw.to(weight.dtype)
-    return dh, dw
-
-
-def _rows_of(t: Tensor | None, rows: slice) -> Tensor | None:
-    return None if t is None else t[rows]
-
-
-class _LinearTokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden: Tensor, weight: Tensor, tokens: Tensor | None, inv_temperature: float,
-                entropy: bool, top: int, ignore_index: int):
-        lead = hidden.shape[:-1]
-        out = _empty_results(lead, hidden.device, tokens, entropy, top)
-        logprobs, h, top_logprobs, top_tokens, stats = out
-        n = stats.shape[0]
-        flat = [None if t is None else t.view(n, *t.shape[len(lead):]) for t in out[:4]] + [stats]
-        t1 = None if tokens is None else tokens.view(-1)
-        for rows, logits in _HeadChunks(hidden, weight):
-            ext().token_logprobs_fwd(logits, _rows_of(t1, rows), inv_temperature, top, ignore_index,
-                                     *(_rows_of(t, rows) for t in flat))
-        ctx.set_materialize_grads(False)
-        if top:
-            ctx.mark_non_differentiable(top_tokens)
-        ctx.save_for_backward(hidden, weight, tokens, top_tokens, stats)
-        ctx.inv_temperature = inv_temperature
-        return logprobs, h, top_logprobs, top_tokens
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_logprobs, d_entropy, d_top, _):
-        hidden, weight, tokens, top_tokens, stats = ctx.saved_tensors
-        if d_logprobs is None and d_entropy is None and d_top is None:
-            return (None,) * 7
-        n = stats.shape[0]
-        g = [None if t is None else _as_f32(t).view(n) for t in (d_logprobs, d_entropy)]
-        g_top = None if d_top is None else _as_f32(d_top).view(n, -1)
-        t1 = None if tokens is None else tokens.view(-1)
-        listed = None if top_tokens is None else top_tokens.view(n, -1)
-
-        def gradient_of(rows, logits, out):
-            ext().token_logprobs_bwd(logits, stats[rows], _rows_of(t1, rows), _rows_of(listed, rows),
-                                     _rows_of(g[0], rows), _rows_of(g[1], rows),
-                                     _rows_of(g_top, rows), ctx.inv_temperature, out)
-
-        dh, dw = _head_backward(ctx, hidden, weight, gradient_of)
-        return dh, dw, None, None, None, None, None
-
-
-class _LinearDistillationFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden: Tensor, weight: Tensor, teacher: Tensor, tokens: Tensor,
-                inv_temperature: float, tail: bool):
-        loss = torch.empty(hidden.shape[:-1], device=hidden.device, dtype=torch.float32)
-        n = loss.numel()
-        stats = torch.empty((n, 4), device=hidden.device, dtype=torch.float32)
-        l1, p1, t1 = loss.view(-1), teacher.view(n, teacher.shape[-1]), tokens.view(n, tokens.shape[-1])
-        for rows, logits in _HeadChunks(hidden, weight):
-            ext().distillation_fwd(logits, p1[rows], t1[rows], inv_temperature, tail, l1[rows],
-                                   stats[rows])
-        ctx.save_for_backward(hidden, weight, p1, t1, stats)
-        ctx.inv_temperature = inv_temperature
-        ctx.tail = tail
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss: Tensor):
-        hidden, weight, teacher, tokens, stats = ctx.saved_tensors
-        g = _as_f32(d_loss).view(-1)
-
-        def gradient_of(rows, logits, out):
-            ext().distillation_bwd(logits, stats[rows], teacher[rows], tokens[rows], g[rows],
-                                   ctx.inv_temperature, ctx.tail, out)
-
-        dh, dw = _head_backward(ctx, hidden, weight, gradient_of)
-        return dh, dw, None, None, None, None
+# The gradient with respect to the logits (bf16), and with a top list the fp32 logits, exist for as many
+# rows at a time as fill this: enough for the products to run at full rate, small next to a training
+# step's activations.
+_CHUNK_BYTES = 1024 * 1024 * 1024
 
 
 def _check_head(hidden: Tensor, weight: Tensor) -> None:
@@ -442,9 +253,10 @@ def linear_token_logprobs(hidden: Tensor, weight: Tensor, tokens: Tensor | None 
                           temperature: float = 1.0, entropy: bool = False, top: int = 0,
                           ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
     """:func:`token_logprobs` of the logits ``hidden @ weight.T`` (``hidden (..., width)``, ``weight
-    (V, width)``), which are made chunk by chunk and not kept; the backward pass makes them again.
-    On the bf16 path (CUDA, bf16 inputs or bf16 autocast) the products run on the tensor cores with
-    fp32 logits; otherwise the logits come from one ``F.linear``."""
+    (V, width)``), which are not kept; the backward pass makes them again. On the bf16 path (CUDA, bf16
+    inputs or bf16 autocast, a width that is a multiple of 8) the statistics are taken from the fp32
+    accumulators of the tensor-core product, and with ``top`` from a gigabyte of fp32 logits at a time;
+    otherwise the logits come from one ``F.linear``."""
     _check_head(hidden, weight)
     temperature = _check_temperature(temperature)
     _check_token_query(hidden.shape[:-1], weight.shape[0], hidden.device, tokens, entropy, top)
@@ -452,9 +264,11 @@ def linear_token_logprobs(hidden: Tensor, weight: Tensor, tokens: Tensor | None 
         return token_logprobs(torch.nn.functional.linear(hidden, weight), tokens,
                               temperature=temperature, entropy=entropy, top=top,
                               ignore_index=ignore_index)
-    tokens = None if tokens is None else _as_tokens(tokens)
-    return TokenLogprobs(*_LinearTokenLogprobsFn.apply(
-        hidden, weight, tokens, 1.0 / temperature, bool(entropy), int(top), int(ignore_index)))
+    from . import bf16_weight
+
+    found = ext().linear_token_logprobs(hidden, weight, bf16_weight(weight), tokens, 1.0 / temperature,
+                                        bool(entropy), top, ignore_index, _CHUNK_BYTES)
+    return _results(found, tokens, entropy, top)
 
 
 def linear_distillation_loss(hidden: Tensor, weight: Tensor, teacher_logprobs: Tensor,
@@ -470,5 +284,7 @@ def linear_distillation_loss(hidden: Tensor, weight: Tensor, teacher_logprobs: T
     if not _fused_head(hidden):
         return distillation_loss(torch.nn.functional.linear(hidden, weight), teacher_logprobs,
                                  teacher_tokens, temperature=temperature, tail=tail)
-    return _LinearDistillationFn.apply(hidden, weight, _as_f32(teacher_logprobs),
-                                       _as_tokens(teacher_tokens), 1.0 / temperature, bool(tail))
+    from . import bf16_weight
+
+    return ext().linear_distillation_loss(hidden, weight, bf16_weight(weight), teacher_logprobs,
+                                          teacher_tokens, 1.0 / temperature, bool(tail), _CHUNK_BYTES)
