@@ -101,7 +101,9 @@ act_quant_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__ 
       amax *= rstd;
     }
     const float clamped = fmaxf(amax, 1e-5f);
-    const float scale = 127.f / clamped;
+    // 127 times the rounded reciprocal, which is how PyTorch evaluates the reference's `127 / amax`:
+    // one rounding in place of two puts entries that lie on a half step on its other side
+    const float scale = __fmul_rn(127.f, __frcp_rn(clamped));
     if (lane == 0) {
       dequant[row] = clamped / 127.f;
       if (HAS_NORM && rstd_out != nullptr) rstd_out[row] = rstd;
