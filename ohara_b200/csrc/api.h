@@ -301,8 +301,9 @@ void linear_token_logprobs(const LinearHead& head, const TokenLogprobsArgs& args
 void linear_distillation(const LinearHead& head, const DistillationArgs& args, float4* partial,
                          float* picked, uint32_t* marks, cudaStream_t stream);
 // d(loss) / d(logits) in bf16 into args.out (pitch a multiple of 8, 16-byte aligned); `picked` from the
-// forward pass, `coef` M elements of scratch. grad_top is not supported here.
-void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool distill,
+// forward pass, `coef` M elements of scratch. With `two`, rows M .. 2 M - 1 of `out` get what the
+// rounding of rows 0 .. M - 1 left. grad_top is not supported here.
+void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool distill, bool two,
                        const float* picked, float4* coef, cudaStream_t stream);
 
 // out (bf16 or fp32) = parts[0] + parts[1] + ... of a product whose reduction was cut in `count` pieces.

@@ -33,6 +33,11 @@ namespace {
 using namespace vocab;
 
 constexpr int kTileM = 256, kTileN = 256, kBlockK = 64;
+// k-blocks that one accumulator sums. The tensor core's running fp32 sum loses a little at every step,
+// always in the same direction; for the statistics, sums of at most 512 terms are added in registers
+// instead, rounded to nearest. Error of a distillation loss at K = 2008: 1.1e-6 with one accumulator,
+// 2.5e-7 so. (The gradient is rounded to bf16 and has no use for it.)
+constexpr int kSegment = 8;
 constexpr int kHalfM = 128;             // rows per CTA of the pair
 constexpr int kRowGroup = 8;            // row tiles that share a pass over the vocabulary
 constexpr int kEpilogueWarps = 8;
@@ -40,13 +45,15 @@ constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 320;
 constexpr int kStageBytes = 2 * kHalfM * kBlockK * 2;  // 128 rows of each operand
 
-enum Mode { kModeSum = kSum, kModeEntropy = kEntropy, kModeSplit = kSplit, kModeGrad };
+// kModeGradPair writes the gradient as a sum of two bf16 matrices, the second below the first.
+enum Mode { kModeSum = kSum, kModeEntropy = kEntropy, kModeSplit = kSplit, kModeGrad, kModeGradPair };
+__host__ __device__ constexpr bool is_grad(Mode m) { return m == kModeGrad || m == kModeGradPair; }
 
 template <Mode MODE>
 struct Layout {
   // the gradient needs two 4 KB staging buffers per epilogue warp
-  static constexpr int kStages = MODE == kModeGrad ? 5 : 6;
-  static constexpr int kStaging = MODE == kModeGrad ? kEpilogueWarps * 2 * 4096 : 0;
+  static constexpr int kStages = is_grad(MODE) ? 5 : 6;
+  static constexpr int kStaging = is_grad(MODE) ? kEpilogueWarps * 2 * 4096 : 0;
   static constexpr int kTotal = kStages * kStageBytes + kStaging + 256 + 1024;
 };
 
@@ -74,7 +81,8 @@ __device__ __forceinline__ void decode(const Params& p, int tile, int& mt, int& 
 template <Mode MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW,
-                  const __grid_constant__ CUtensorMap tmD, const Params p) {
+                  const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmRest,
+                  const Params p) {
   using L = Layout<MODE>;
   constexpr int kStages = L::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -95,6 +103,8 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
   const int total_tiles = p.m_tiles * p.n_tiles;
   const int first_tile = (int)(blockIdx.x >> 1), tile_step = (int)(gridDim.x >> 1);
   const int k_blocks = (p.K + kBlockK - 1) / kBlockK;
+  const int segments = is_grad(MODE) ? 1 : (k_blocks + kSegment - 1) / kSegment;
+  const int per_segment = (k_blocks + segments - 1) / segments;  // the last may be shorter, not empty
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -111,7 +121,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
   if (warp == kProducerWarp && lane == 0) {
     prefetch_tmap(&tmH);
     prefetch_tmap(&tmW);
-    if (MODE == kModeGrad) prefetch_tmap(&tmD);
+    if (is_grad(MODE)) prefetch_tmap(&tmD);
   }
   if (warp == kMmaWarp) {
     tmem_alloc_pair(tmem_slot, 2 * kTileN);
@@ -156,41 +166,48 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
       const uint32_t idesc = make_idesc_bf16(kTileM, kTileN, false, false);
       const SmemDesc desc_h = make_smem_desc_parts(smem_u32(smem), 16, 1024);
       const SmemDesc desc_w = make_smem_desc_parts(smem_u32(smem + kHalfM * kBlockK * 2), 16, 1024);
-      uint32_t it = 0, tile_iter = 0;
+      uint32_t it = 0, acc_iter = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step, ++tile_iter) {
-        const uint32_t acc = tile_iter & 1;
-        if (!mbar_wait(&tmem_empty[acc], ((tile_iter >> 1) & 1) ^ 1, wctx, kTimeoutTmemEmpty)) break;
-        tcgen05_fence_after();
-        const uint32_t tmem_acc = tmem_base + acc * kTileN;
-        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&full_bar[s], (it / kStages) & 1, wctx, kTimeoutFullBarrier)) {
+      for (int tile = first_tile; tile < total_tiles && ok; tile += tile_step) {
+        for (int begin = 0; begin < k_blocks && ok; begin += per_segment, ++acc_iter) {
+          const int end = min(begin + per_segment, k_blocks);
+          const uint32_t acc = acc_iter & 1;
+          if (!mbar_wait(&tmem_empty[acc], ((acc_iter >> 1) & 1) ^ 1, wctx, kTimeoutTmemEmpty)) {
             ok = false;
             break;
           }
           tcgen05_fence_after();
+          const uint32_t tmem_acc = tmem_base + acc * kTileN;
+          for (int kb = begin; kb < end; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait(&full_bar[s], (it / kStages) & 1, wctx, kTimeoutFullBarrier)) {
+              ok = false;
+              break;
+            }
+            tcgen05_fence_after();
 #pragma unroll
-          for (int k = 0; k < kBlockK / 16; ++k)
-            umma_bf16_ss_pair(tmem_acc, smem_desc_at(desc_h, s * kStageBytes + k * 32),
-                              smem_desc_at(desc_w, s * kStageBytes + k * 32), idesc,
-                              (kb > 0 || k > 0) ? 1u : 0u);
-          const uint32_t addr = smem_u32(&empty_bar[s]);  // frees the stage in both CTAs
+            for (int k = 0; k < kBlockK / 16; ++k)
+              umma_bf16_ss_pair(tmem_acc, smem_desc_at(desc_h, s * kStageBytes + k * 32),
+                                smem_desc_at(desc_w, s * kStageBytes + k * 32), idesc,
+                                (kb > begin || k > 0) ? 1u : 0u);
+            const uint32_t addr = smem_u32(&empty_bar[s]);  // frees the stage in both CTAs
+            tcgen05_commit_pair(map_to_cta(addr, 0));
+            tcgen05_commit_pair(map_to_cta(addr, 1));
+          }
+          if (!ok) break;
+          const uint32_t addr = smem_u32(&tmem_full[acc]);
           tcgen05_commit_pair(map_to_cta(addr, 0));
           tcgen05_commit_pair(map_to_cta(addr, 1));
         }
-        if (!ok) break;
-        const uint32_t addr = smem_u32(&tmem_full[acc]);
-        tcgen05_commit_pair(map_to_cta(addr, 0));
-        tcgen05_commit_pair(map_to_cta(addr, 1));
       }
     }
   } else {
     // ------------------------------- Epilogue ----------------------------------------------------
     const int quarter = warp & 3, half = warp >> 2;
-    uint32_t tile_iter = 0, store_iter = 0;
+    uint32_t acc_iter = 0, store_iter = 0;
+    bool ok = true;
     const uint64_t c2 = pair(p.c, p.c);
-    for (int tile = first_tile; tile < total_tiles; tile += tile_step, ++tile_iter) {
+    for (int tile = first_tile; tile < total_tiles; tile += tile_step) {
       int mt, nt;
       decode(p, tile, mt, nt);
       const int row0 = mt * kTileM + (int)cta_rank * kHalfM + quarter * 32;
@@ -201,22 +218,43 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
       if (row < p.M) {
         if (MODE == kModeSplit)
           words = *reinterpret_cast<const uint4*>(p.marks + ((int64_t)row * p.n_tiles + nt) * 8 + half * 4);
-        if (MODE == kModeGrad) coef = p.coef[row];
+        if (is_grad(MODE)) coef = p.coef[row];
       }
-      const uint32_t acc = tile_iter & 1;
-      if (!mbar_wait(&tmem_full[acc], (tile_iter >> 1) & 1, wctx, kTimeoutTmemFull)) break;
-      tcgen05_fence_after();
-      const uint32_t taddr =
-          tmem_base + acc * kTileN + half * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
       uint32_t v[4][32];
+#pragma unroll 1
+      for (int segment = 0; segment < segments; ++segment, ++acc_iter) {
+        const uint32_t acc = acc_iter & 1;
+        if (!mbar_wait(&tmem_full[acc], (acc_iter >> 1) & 1, wctx, kTimeoutTmemFull)) {
+          ok = false;
+          break;
+        }
+        tcgen05_fence_after();
+        const uint32_t taddr =
+            tmem_base + acc * kTileN + half * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
+        if (is_grad(MODE) || segment == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld_32x32(taddr + 32 * i, v[i]);
-      tmem_ld_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty[acc]), 0));
+          for (int i = 0; i < 4; ++i) tmem_ld_32x32(taddr + 32 * i, v[i]);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t more[16];
+            tmem_ld_32x16(taddr + 16 * i, more);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              uint32_t& sum = v[i >> 1][16 * (i & 1) + j];
+              sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(more[j]));
+            }
+          }
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty[acc]), 0));
+      }
+      if (!ok) break;
 
-      if constexpr (MODE != kModeGrad) {
+      if constexpr (!is_grad(MODE)) {
         const int cols = p.N - col0;  // columns of this half that exist
         if (cols < 128) {
 #pragma unroll
@@ -267,10 +305,23 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
 #pragma unroll
         for (int part = 0; part < 2; ++part) {  // 64 columns: 128 bytes a row
           if (col0 + 64 * part >= p.N) break;   // uniform over the warp
-          uint8_t* buf = my_staging + (store_iter & 1) * 4096;
-          ++store_iter;
-          if (lane == 0) tma_store_wait_read<1>();
-          __syncwarp();
+          auto next_buffer = [&] {
+            uint8_t* buf = my_staging + (store_iter & 1) * 4096;
+            ++store_iter;
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+            return buf;
+          };
+          auto send = [&](const CUtensorMap* map, uint8_t* buf) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (row0 < p.M) tma_store_3d(map, buf, col0 + 64 * part, row0, 0);
+              tma_store_commit();
+            }
+          };
+          uint32_t rest[MODE == kModeGradPair ? 32 : 1];
+          uint8_t* buf = next_buffer();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {  // 16 bytes
             uint32_t packed[4];
@@ -278,7 +329,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
             for (int r = 0; r < 4; ++r) {
               const int col = 64 * part + 8 * q + 2 * r;
               const uint64_t x = pair(__uint_as_float(v[col >> 5][col & 31]),
-                                       __uint_as_float(v[col >> 5][(col & 31) + 1]));
+                                      __uint_as_float(v[col >> 5][(col & 31) + 1]));
               float2 t = both(mul2(add2(x, ref2), c2));
               // e is 0 from t = -150 down; the clamp keeps slope t finite (and drops NaN where the
               // reference is +inf: a row that nothing asks for gets zeros whatever its logits)
@@ -286,20 +337,26 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
               const uint64_t e = pair(fast_exp2(t.x), fast_exp2(t.y));
               const float2 d = both(mul2(e, fma2(slope2, pair(t.x, t.y), level2)));
               packed[r] = pack_bf16(d.x, d.y);
+              if constexpr (MODE == kModeGradPair)
+                rest[4 * q + r] = pack_bf16(d.x - __uint_as_float(packed[r] << 16),
+                                            d.y - __uint_as_float(packed[r] & 0xffff0000u));
             }
             *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
                 make_uint4(packed[0], packed[1], packed[2], packed[3]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (row0 < p.M) tma_store_3d(&tmD, buf, col0 + 64 * part, row0, 0);
-            tma_store_commit();
+          send(&tmD, buf);
+          if constexpr (MODE == kModeGradPair) {
+            buf = next_buffer();
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                  make_uint4(rest[4 * q], rest[4 * q + 1], rest[4 * q + 2], rest[4 * q + 3]);
+            send(&tmRest, buf);
           }
         }
       }
     }
-    if (MODE == kModeGrad && lane == 0) tma_store_wait_all<0>();
+    if (is_grad(MODE) && lane == 0) tma_store_wait_all<0>();
   }
 
   // ------------------------------- Teardown ---------------------------------------------------
@@ -318,8 +375,8 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant
 }
 
 template <Mode MODE>
-void launch_gemm(const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& d, const Params& p,
-                 cudaStream_t stream) {
+void launch_gemm(const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& d,
+                 const CUtensorMap& rest, const Params& p, cudaStream_t stream) {
   using L = Layout<MODE>;
   auto kernel = vocab_gemm_kernel<MODE>;
   static int resident_by_device[64] = {0};
@@ -347,7 +404,7 @@ void launch_gemm(const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& 
   }
   const int pairs = (int)std::min<long long>((long long)p.m_tiles * p.n_tiles, resident);
   config.gridDim = dim3(2 * pairs, 1, 1);
-  OB_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, h, w, d, p));
+  OB_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, h, w, d, rest, p));
   count_launch();
 }
 
@@ -531,7 +588,7 @@ grad_coefficients_kernel(const VocabGradArgs p, float4* coef, int M) {
 template <bool DISTILL>
 __global__ void __launch_bounds__(256)
 grad_named_kernel(const VocabGradArgs p, const float4* coef, const float* picked, __nv_bfloat16* out,
-                  int64_t pitch, int M) {
+                  int64_t pitch, int M, int two) {
   const int per_row = DISTILL ? p.top : 1;
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= (int64_t)M * per_row) return;
@@ -554,7 +611,10 @@ grad_named_kernel(const VocabGradArgs p, const float4* coef, const float* picked
   }
   if (!first) return;
   const float t = grad_exponent(picked[e], g.x, p.inv_temperature * kLog2e);
-  out[row * pitch + token] = __float2bfloat16_rn(fast_exp2(t) * fmaf(g.z, t, g.w) + weight);
+  const float d = fast_exp2(t) * fmaf(g.z, t, g.w) + weight;
+  const __nv_bfloat16 first_part = __float2bfloat16_rn(d);
+  out[row * pitch + token] = first_part;
+  if (two) out[(row + M) * pitch + token] = __float2bfloat16_rn(d - __bfloat162float(first_part));
 }
 
 // out = sum of the parts, in order; four elements a thread.
@@ -647,11 +707,11 @@ void linear_token_logprobs(const LinearHead& head, const TokenLogprobsArgs& args
   if (args.logprobs != nullptr) pick_logits(head, args.tokens, picked, 1, stream);
   const unsigned blocks = (unsigned)((head.M + kJoinRows - 1) / kJoinRows);
   if (args.entropy != nullptr) {
-    launch_gemm<kModeEntropy>(plan.h, plan.w, plan.w, plan.p, stream);
+    launch_gemm<kModeEntropy>(plan.h, plan.w, plan.w, plan.w, plan.p, stream);
     join_logprobs_kernel<kEntropy><<<blocks, kJoinWarps * 32, 0, stream>>>(partial, halves, pitch,
                                                                           head.M, picked, args);
   } else {
-    launch_gemm<kModeSum>(plan.h, plan.w, plan.w, plan.p, stream);
+    launch_gemm<kModeSum>(plan.h, plan.w, plan.w, plan.w, plan.p, stream);
     join_logprobs_kernel<kSum><<<blocks, kJoinWarps * 32, 0, stream>>>(partial, halves, pitch, head.M,
                                                                       picked, args);
   }
@@ -674,24 +734,29 @@ void linear_distillation(const LinearHead& head, const DistillationArgs& args, f
         args.tokens, marks, entries, args.top, head.N, words);
     OB_LAUNCH_CHECK();
     plan.p.marks = marks;
-    launch_gemm<kModeSplit>(plan.h, plan.w, plan.w, plan.p, stream);
+    launch_gemm<kModeSplit>(plan.h, plan.w, plan.w, plan.w, plan.p, stream);
     join_distillation_kernel<true><<<blocks, kJoinWarps * 32, 0, stream>>>(partial, halves, pitch,
                                                                             head.M, picked, args);
   } else {
-    launch_gemm<kModeSum>(plan.h, plan.w, plan.w, plan.p, stream);
+    launch_gemm<kModeSum>(plan.h, plan.w, plan.w, plan.w, plan.p, stream);
     join_distillation_kernel<false><<<blocks, kJoinWarps * 32, 0, stream>>>(partial, halves, pitch,
                                                                           head.M, picked, args);
   }
   OB_LAUNCH_CHECK();
 }
 
-void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool distill,
+void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool distill, bool two,
                        const float* picked, float4* coef, cudaStream_t stream) {
   Plan plan = make_plan(head, args.inv_temperature);
   plan.p.coef = coef;
-  CUtensorMap d;
-  make_tmap_3d(&d, args.out, TmapDtype::BF16, (uint64_t)head.N, (uint64_t)head.M, 1, args.out_pitch, 0,
-               64, 32, TmapSwizzle::B128);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(args.out);
+  CUtensorMap d, rest;
+  auto map = [&](CUtensorMap* m, void* base) {
+    make_tmap_3d(m, base, TmapDtype::BF16, (uint64_t)head.N, (uint64_t)head.M, 1, args.out_pitch, 0, 64, 32,
+                 TmapSwizzle::B128);
+  };
+  map(&d, out);
+  map(&rest, two ? out + head.M * args.out_pitch : out);
   const unsigned rows = (unsigned)((head.M + 255) / 256);
   const int64_t entries = (int64_t)head.M * (distill ? args.top : 1);
   const unsigned named = (unsigned)((entries + 255) / 256);
@@ -700,13 +765,14 @@ void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool d
   else
     grad_coefficients_kernel<false><<<rows, 256, 0, stream>>>(args, coef, head.M);
   OB_LAUNCH_CHECK();
-  launch_gemm<kModeGrad>(plan.h, plan.w, d, plan.p, stream);
+  if (two)
+    launch_gemm<kModeGradPair>(plan.h, plan.w, d, rest, plan.p, stream);
+  else
+    launch_gemm<kModeGrad>(plan.h, plan.w, d, rest, plan.p, stream);
   if (distill)
-    grad_named_kernel<true><<<named, 256, 0, stream>>>(args, coef, picked, (__nv_bfloat16*)args.out,
-                                                       args.out_pitch, head.M);
+    grad_named_kernel<true><<<named, 256, 0, stream>>>(args, coef, picked, out, args.out_pitch, head.M, two);
   else if (args.grad != nullptr)
-    grad_named_kernel<false><<<named, 256, 0, stream>>>(args, coef, picked, (__nv_bfloat16*)args.out,
-                                                        args.out_pitch, head.M);
+    grad_named_kernel<false><<<named, 256, 0, stream>>>(args, coef, picked, out, args.out_pitch, head.M, two);
   else
     return;
   OB_LAUNCH_CHECK();

@@ -424,13 +424,19 @@ int64_t reduction_cuts(int64_t rows, int64_t width, int64_t vocab) {
   return best;
 }
 
-// dh (rows x width) = d W, the pieces added in a fixed order.
-void hidden_gradient(const Head& h, const Tensor& d, int64_t rows, int64_t pitch, const Tensor& dh,
-                     int64_t first) {
+// Up to this many rows the gradient with respect to the logits is held as the sum of two bf16 matrices:
+// the products are bound by the weight then, and with few rows the rounding of single elements (the
+// target's, near 1) shows in the results: error 2.7e-3 against 1.7e-3 of the results' own rounding at
+// 4 x 1256, 1.7e-3 with the pair.
+constexpr int64_t kPairRows = 256;
+
+// dh (n x width) = sum over the `copies` blocks of n rows in d of d W, the pieces added in a fixed order.
+void hidden_gradient(const Head& h, const Tensor& d, int64_t n, int64_t copies, int64_t pitch,
+                     const Tensor& dh, int64_t first) {
   char* out = static_cast<char*>(dh.data_ptr()) + 2 * first * h.width;
-  const int64_t ldw = pitch_of(h.weight);
+  const int64_t ldw = pitch_of(h.weight), rows = n * copies;
   const int64_t cuts = reduction_cuts(rows, h.width, h.vocab);
-  if (cuts == 1) {
+  if (cuts * copies == 1) {
     gemm(d.data_ptr(), h.weight.data_ptr(), out, rows, h.width, h.vocab, 1, false, pitch, ldw, h.width, 0, 0,
          0, false, false);
     return;
@@ -440,22 +446,24 @@ void hidden_gradient(const Head& h, const Tensor& d, int64_t rows, int64_t pitch
   const int64_t count = whole + (rest > 0 ? 1 : 0);
   Tensor parts = f32(d, {count, rows, h.width});
   float* p = parts.data_ptr<float>();
-  gemm(d.data_ptr(), h.weight.data_ptr(), p, rows, h.width, piece, whole, false, pitch, ldw, h.width, piece,
-       piece * ldw, rows * h.width, true, false);
+  if (whole > 0)
+    gemm(d.data_ptr(), h.weight.data_ptr(), p, rows, h.width, piece, whole, false, pitch, ldw, h.width, piece,
+         piece * ldw, rows * h.width, true, false);
   if (rest > 0)
     gemm(static_cast<char*>(d.data_ptr()) + 2 * whole * piece,
          static_cast<char*>(h.weight.data_ptr()) + 2 * whole * piece * ldw, p + whole * rows * h.width, rows,
          h.width, rest, 1, false, pitch, ldw, h.width, 0, 0, 0, true, false);
-  ob::sum_parts(p, out, false, rows * h.width, (int)count, current_stream());
+  ob::sum_parts(p, out, false, n * h.width, (int)(count * copies), current_stream());
 }
 
-// Gradients of hidden states and weight from `gradient(first, rows, out, pitch)`, which writes
-// d(loss) / d(logits) of some rows in bf16, the operand type of the two products that follow; both
-// accumulate in fp32, the weight's over all chunks and in a fixed order.
-using GradientOf = std::function<void(int64_t, int64_t, const Tensor&, int64_t)>;
+// Gradients of hidden states and weight from `gradient(first, rows, out, pitch, two)`, which writes
+// d(loss) / d(logits) of some rows in bf16, the operand type of the two products that follow (with
+// `two` as a pair, see kPairRows); both accumulate in fp32, the weight's over all chunks and in a fixed
+// order.
+using GradientOf = std::function<void(int64_t, int64_t, const Tensor&, int64_t, bool)>;
 std::pair<Tensor, Tensor> head_backward(const Head& h, at::IntArrayRef hidden_sizes,
                                         torch::ScalarType hidden_type, torch::ScalarType weight_type,
-                                        bool need_dh, bool need_dw, int64_t chunk_bytes,
+                                        bool need_dh, bool need_dw, bool pairs, int64_t chunk_bytes,
                                         const GradientOf& gradient) {
   const auto options = h.hidden.options();
   Tensor dh, dw;
@@ -466,7 +474,11 @@ std::pair<Tensor, Tensor> head_backward(const Head& h, at::IntArrayRef hidden_si
   }
   const int64_t step = chunk_rows(h, 2 * h.vocab, chunk_bytes);
   const int64_t pitch = (h.vocab + 7) / 8 * 8;
-  Tensor d = torch::empty({step, pitch}, options);
+  const bool two = pairs && h.n <= kPairRows;
+  const int64_t copies = two ? 2 : 1;
+  Tensor d = torch::empty({copies * step, pitch}, options);
+  const Tensor hidden = two && need_dw ? torch::cat({h.hidden, h.hidden}) : h.hidden;
+  const int64_t ldh = pitch_of(hidden);
   if (need_dh) dh = torch::empty({h.n, h.width}, options);
   if (need_dw)  // the product of a single chunk can be rounded to the weight's type as it is written
     dw = torch::empty({h.vocab, h.width},
@@ -474,14 +486,12 @@ std::pair<Tensor, Tensor> head_backward(const Head& h, at::IntArrayRef hidden_si
                                                                                    : torch::kFloat32));
   for (int64_t first = 0; first < h.n; first += step) {
     const int64_t rows = std::min(step, h.n - first);
-    gradient(first, rows, d, pitch);
-    if (need_dh) hidden_gradient(h, d, rows, pitch, dh, first);
-    if (need_dw) {
-      const int64_t ldh = pitch_of(h.hidden);
-      gemm(d.data_ptr(), static_cast<char*>(h.hidden.data_ptr()) + 2 * first * ldh, dw.data_ptr(), h.vocab,
-           h.width, rows, 1, true, pitch, ldh, h.width, 0, 0, 0, dw.scalar_type() == torch::kFloat32,
+    gradient(first, rows, d, pitch, two);
+    if (need_dh) hidden_gradient(h, d, rows, copies, pitch, dh, first);
+    if (need_dw)
+      gemm(d.data_ptr(), static_cast<char*>(hidden.data_ptr()) + 2 * first * ldh, dw.data_ptr(), h.vocab,
+           h.width, rows * copies, 1, true, pitch, ldh, h.width, 0, 0, 0, dw.scalar_type() == torch::kFloat32,
            first > 0);
-    }
   }
   if (need_dh) dh = dh.view(hidden_sizes).to(hidden_type);
   if (need_dw) dw = dw.to(weight_type);
@@ -581,7 +591,7 @@ struct LinearTokenLogprobsFn : torch::autograd::Function<LinearTokenLogprobsFn> 
     const double inv = ctx->saved_data["inv"].toDouble();
     const int64_t chunk = ctx->saved_data["chunk"].toInt();
     Tensor coef = f32(hidden, {chunk_rows(h, 2 * h.vocab, chunk), 4});
-    auto gradient = [&](int64_t first, int64_t rows, const Tensor& d, int64_t pitch) {
+    auto gradient = [&](int64_t first, int64_t rows, const Tensor& d, int64_t pitch, bool two) {
       if (top_tokens.defined()) {
         over_logits(h, first, rows, chunk, [&](const LogitRows& l, int64_t at) {
           run_logprobs_grad(l, stats, tokens, top_tokens, g, inv, at, d.narrow(0, at - first, l.rows), pitch);
@@ -598,12 +608,13 @@ struct LinearTokenLogprobsFn : torch::autograd::Function<LinearTokenLogprobsFn> 
       a.tokens = at_row(data<int64_t>(tokens));
       a.inv_temperature = (float)inv;
       a.vocab = (int)h.vocab;
-      ob::linear_vocab_grad(h.part(first, rows), a, false, at_row(data<float>(picked)), stats_of(coef),
-                            current_stream());
+      ob::linear_vocab_grad(h.part(first, rows), a, false, two, at_row(data<float>(picked)),
+                            stats_of(coef), current_stream());
     };
     std::tie(out[0], out[1]) =
         head_backward(h, hidden.sizes(), hidden.scalar_type(), weight.scalar_type(),
-                      ctx->needs_input_grad(0), ctx->needs_input_grad(1), chunk, gradient);
+                      ctx->needs_input_grad(0), ctx->needs_input_grad(1), !top_tokens.defined(), chunk,
+                      gradient);
     return once(std::move(out));
   }
 };
@@ -674,19 +685,19 @@ struct LinearDistillationFn : torch::autograd::Function<LinearDistillationFn> {
     const Tensor g = grads[0].to(torch::kFloat32).contiguous();
     const int64_t chunk = ctx->saved_data["chunk"].toInt();
     Tensor coef = f32(hidden, {chunk_rows(h, 2 * h.vocab, chunk), 4});
-    auto gradient = [&](int64_t first, int64_t rows, const Tensor& d, int64_t pitch) {
+    auto gradient = [&](int64_t first, int64_t rows, const Tensor& d, int64_t pitch, bool two) {
       ob::VocabGradArgs a =
           distillation_grad_args(teacher, tokens, stats, g, ctx->saved_data["inv"].toDouble(),
                                  ctx->saved_data["tail"].toBool(), (int)h.vocab, first);
       a.out = d.data_ptr();
       a.out_pitch = pitch;
-      ob::linear_vocab_grad(h.part(first, rows), a, true, data<float>(picked) + first * a.top,
+      ob::linear_vocab_grad(h.part(first, rows), a, true, two, data<float>(picked) + first * a.top,
                             stats_of(coef), current_stream());
     };
     variable_list out(8);
     std::tie(out[0], out[1]) =
         head_backward(h, hidden.sizes(), hidden.scalar_type(), weight.scalar_type(),
-                      ctx->needs_input_grad(0), ctx->needs_input_grad(1), chunk, gradient);
+                      ctx->needs_input_grad(0), ctx->needs_input_grad(1), true, chunk, gradient);
     return once(std::move(out));
   }
 };
