@@ -269,8 +269,7 @@ void distillation_loss(const RowsView& view, LogitType type, DistillationArgs ar
 // Gradient with respect to the logits of either of the two, from the `stats` that it left.
 struct VocabGradArgs {
   const float4* stats;
-  void* out;              // (rows, out_pitch)
-  int64_t out_pitch;
+  RowsView out;               // where the rows go (its `base` is written to)
   const float* grad;          // (rows): of the log-probabilities (or null) / of the loss
   const float* grad_entropy;  // (rows) or null
   const float* grad_top;      // (rows, top) or null
@@ -300,7 +299,7 @@ void linear_token_logprobs(const LinearHead& head, const TokenLogprobsArgs& args
                            float* picked, cudaStream_t stream);
 void linear_distillation(const LinearHead& head, const DistillationArgs& args, float4* partial,
                          float* picked, uint32_t* marks, cudaStream_t stream);
-// d(loss) / d(logits) in bf16 into args.out (pitch a multiple of 8, 16-byte aligned); `picked` from the
+// d(loss) / d(logits) in bf16 into args.out (one row pitch, a multiple of 8; 16-byte aligned); `picked` from the
 // forward pass, `coef` M elements of scratch. With `two`, rows M .. 2 M - 1 of `out` get what the
 // rounding of rows 0 .. M - 1 left. grad_top is not supported here.
 void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool distill, bool two,

@@ -749,14 +749,15 @@ void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool d
                        const float* picked, float4* coef, cudaStream_t stream) {
   Plan plan = make_plan(head, args.inv_temperature);
   plan.p.coef = coef;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(args.out);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(const_cast<void*>(args.out.base));
+  const int64_t pitch = args.out.inner_stride;
   CUtensorMap d, rest;
   auto map = [&](CUtensorMap* m, void* base) {
-    make_tmap_3d(m, base, TmapDtype::BF16, (uint64_t)head.N, (uint64_t)head.M, 1, args.out_pitch, 0, 64, 32,
+    make_tmap_3d(m, base, TmapDtype::BF16, (uint64_t)head.N, (uint64_t)head.M, 1, pitch, 0, 64, 32,
                  TmapSwizzle::B128);
   };
   map(&d, out);
-  map(&rest, two ? out + head.M * args.out_pitch : out);
+  map(&rest, two ? out + head.M * pitch : out);
   const unsigned rows = (unsigned)((head.M + 255) / 256);
   const int64_t entries = (int64_t)head.M * (distill ? args.top : 1);
   const unsigned named = (unsigned)((entries + 255) / 256);
@@ -770,9 +771,9 @@ void linear_vocab_grad(const LinearHead& head, const VocabGradArgs& args, bool d
   else
     launch_gemm<kModeGrad>(plan.h, plan.w, d, rest, plan.p, stream);
   if (distill)
-    grad_named_kernel<true><<<named, 256, 0, stream>>>(args, coef, picked, out, args.out_pitch, head.M, two);
+    grad_named_kernel<true><<<named, 256, 0, stream>>>(args, coef, picked, out, pitch, head.M, two);
   else if (args.grad != nullptr)
-    grad_named_kernel<false><<<named, 256, 0, stream>>>(args, coef, picked, out, args.out_pitch, head.M, two);
+    grad_named_kernel<false><<<named, 256, 0, stream>>>(args, coef, picked, out, pitch, head.M, two);
   else
     return;
   OB_LAUNCH_CHECK();

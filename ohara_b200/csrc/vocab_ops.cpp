@@ -83,6 +83,29 @@ LogitRows logit_rows(const Tensor& logits) {
   return r;
 }
 
+ob::RowsView pitched(void* base, int64_t pitch, int64_t rows) { return ob::RowsView{base, 0, pitch, rows}; }
+
+// A tensor for the gradient of `logits`, in their layout if that has no more than a few gaps: its rows
+// then start at the same distance from a 16-byte boundary and whole vectors can be stored (a slice of
+// a padded or odd vocabulary, `logits[:, :-1]`).
+Tensor gradient_like(const Tensor& logits, const LogitRows& l, ob::RowsView& view) {
+  const int64_t item = logits.element_size();
+  const int64_t offset = reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16 / item;
+  const ob::RowsView& v = l.view;
+  const int64_t outer = l.rows > 0 ? l.rows / v.inner : 0;
+  const int64_t span = (outer - 1) * v.outer_stride + (v.inner - 1) * v.inner_stride + l.vocab;
+  const bool apart = (v.inner <= 1 || v.inner_stride >= l.vocab) &&
+                     (outer <= 1 || v.outer_stride >= (v.inner - 1) * v.inner_stride + l.vocab);
+  Tensor out;
+  if (l.rows > 0 && l.t.is_same(logits) && apart && span <= 2 * logits.numel() &&
+      (offset != 0 || !logits.is_contiguous()))
+    out = torch::empty({offset + span}, logits.options()).as_strided(logits.sizes(), logits.strides(), offset);
+  else
+    out = torch::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+  TORCH_CHECK(rows_view(out, view));
+  return out;
+}
+
 template <typename S>
 S* data(const Tensor& t) {
   return t.defined() ? t.data_ptr<S>() : nullptr;
@@ -198,13 +221,12 @@ struct TokenGrads {
 
 void run_logprobs_grad(const LogitRows& l, const Tensor& stats, const Tensor& tokens,
                        const Tensor& top_tokens, const TokenGrads& g, double inv_temperature,
-                       int64_t first, const Tensor& out, int64_t out_pitch) {
+                       int64_t first, ob::LogitType out_type, const ob::RowsView& out) {
   ob::VocabGradArgs a = {};
   auto at_row = [&](auto* p, int64_t width) { return p == nullptr ? nullptr : p + first * width; };
   const int64_t top = g.top.defined() ? g.top.size(-1) : 0;
   a.stats = stats_of(stats) + first;
-  a.out = out.data_ptr();
-  a.out_pitch = out_pitch;
+  a.out = out;
   a.grad = at_row(data<float>(g.logprobs), 1);
   a.grad_entropy = at_row(data<float>(g.entropy), 1);
   a.grad_top = at_row(data<float>(g.top), top);
@@ -213,7 +235,7 @@ void run_logprobs_grad(const LogitRows& l, const Tensor& stats, const Tensor& to
   a.inv_temperature = (float)inv_temperature;
   a.vocab = l.vocab;
   a.top = (int)top;
-  ob::vocab_grad(l.view, l.type, logit_type(out), a, l.rows, false, current_stream());
+  ob::vocab_grad(l.view, l.type, out_type, a, l.rows, false, current_stream());
 }
 
 struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
@@ -245,8 +267,9 @@ struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
     if (!g.any()) return out;
     const c10::cuda::CUDAGuard guard(logits.device());
     const LogitRows l = logit_rows(logits);
-    out[0] = torch::empty(logits.sizes(), logits.options());
-    run_logprobs_grad(l, stats, tokens, top_tokens, g, ctx->saved_data["inv"].toDouble(), 0, out[0], l.vocab);
+    ob::RowsView to;
+    out[0] = gradient_like(logits, l, to);
+    run_logprobs_grad(l, stats, tokens, top_tokens, g, ctx->saved_data["inv"].toDouble(), 0, l.type, to);
     return once(std::move(out));
   }
 };
@@ -321,13 +344,13 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
     const LogitRows l = logit_rows(logits);
     const Tensor g = grads[0].to(torch::kFloat32).contiguous();
     variable_list out(5);
-    out[0] = torch::empty(logits.sizes(), logits.options());
+    ob::RowsView to;
+    out[0] = gradient_like(logits, l, to);
     if (l.rows > 0) {
       ob::VocabGradArgs a =
           distillation_grad_args(saved[1], saved[2], saved[3], g, ctx->saved_data["inv"].toDouble(),
                                  ctx->saved_data["tail"].toBool(), l.vocab, 0);
-      a.out = out[0].data_ptr();
-      a.out_pitch = l.vocab;
+      a.out = to;
       ob::vocab_grad(l.view, l.type, l.type, a, l.rows, true, current_stream());
     }
     return once(std::move(out));
@@ -513,7 +536,7 @@ void over_logits(const Head& h, int64_t first, int64_t rows, int64_t chunk_bytes
                   ob::device_sm_count(), nullptr, 0, 0, 0.f, current_stream());
     LogitRows l;
     l.t = logits;
-    l.view = ob::RowsView{logits.data_ptr(), 0, pitch, n};
+    l.view = pitched(logits.data_ptr(), pitch, n);
     l.type = ob::LogitType::F32;
     l.rows = n;
     l.vocab = (int)h.vocab;
@@ -594,15 +617,15 @@ struct LinearTokenLogprobsFn : torch::autograd::Function<LinearTokenLogprobsFn> 
     auto gradient = [&](int64_t first, int64_t rows, const Tensor& d, int64_t pitch, bool two) {
       if (top_tokens.defined()) {
         over_logits(h, first, rows, chunk, [&](const LogitRows& l, int64_t at) {
-          run_logprobs_grad(l, stats, tokens, top_tokens, g, inv, at, d.narrow(0, at - first, l.rows), pitch);
+          run_logprobs_grad(l, stats, tokens, top_tokens, g, inv, at, ob::LogitType::BF16,
+                            pitched(static_cast<char*>(d.data_ptr()) + 2 * (at - first) * pitch, pitch, l.rows));
         });
         return;
       }
       auto at_row = [&](auto* p) { return p == nullptr ? nullptr : p + first; };
       ob::VocabGradArgs a = {};
       a.stats = stats_of(stats) + first;
-      a.out = d.data_ptr();
-      a.out_pitch = pitch;
+      a.out = pitched(d.data_ptr(), pitch, rows);
       a.grad = at_row(data<float>(g.logprobs));
       a.grad_entropy = at_row(data<float>(g.entropy));
       a.tokens = at_row(data<int64_t>(tokens));
@@ -689,8 +712,7 @@ struct LinearDistillationFn : torch::autograd::Function<LinearDistillationFn> {
       ob::VocabGradArgs a =
           distillation_grad_args(teacher, tokens, stats, g, ctx->saved_data["inv"].toDouble(),
                                  ctx->saved_data["tail"].toBool(), (int)h.vocab, first);
-      a.out = d.data_ptr();
-      a.out_pitch = pitch;
+      a.out = pitched(d.data_ptr(), pitch, rows);
       ob::linear_vocab_grad(h.part(first, rows), a, true, two, data<float>(picked) + first * a.top,
                             stats_of(coef), current_stream());
     };

@@ -898,7 +898,7 @@ vocab_grad_kernel(const RowsView view, const VocabGradArgs p) {
   const int vocab = p.vocab;
   const float c = p.inv_temperature * kLog2e;
   const T* x = row_of<T>(view, row);
-  O* out = static_cast<O*>(p.out) + row * p.out_pitch;
+  O* out = const_cast<O*>(row_of<O>(p.out, row));
   const Slice sl = slice_of(x, vocab, part, p.parts);
   const int edge = edge_index(sl, vocab, part);
 

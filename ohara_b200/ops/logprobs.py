@@ -47,9 +47,8 @@ class TokenLogprobs(NamedTuple):
 # --------------------------------------------------------------------------------------------------
 # Reference expressions
 # --------------------------------------------------------------------------------------------------
-def _scaled_log_softmax(logits: Tensor, temperature: float) -> Tensor:
-    wide = logits if logits.dtype == torch.float64 else logits.float()
-    return torch.log_softmax(wide / temperature, dim=-1)
+def _scaled(logits: Tensor, temperature: float) -> Tensor:
+    return (logits if logits.dtype == torch.float64 else logits.float()) / temperature
 
 
 def _nan_where(bad: Tensor, like: Tensor) -> Tensor:
@@ -60,7 +59,7 @@ def _nan_where(bad: Tensor, like: Tensor) -> Tensor:
 def token_logprobs_reference(logits: Tensor, tokens: Tensor | None = None, *,
                              temperature: float = 1.0, entropy: bool = False, top: int = 0,
                              ignore_index: int = IGNORE_INDEX) -> TokenLogprobs:
-    logq = _scaled_log_softmax(logits, temperature)
+    logq = torch.log_softmax(_scaled(logits, temperature), dim=-1)
     keep = torch.ones(logits.shape[:-1], dtype=torch.bool, device=logits.device)
     picked = h = top_logprobs = top_tokens = None
     if tokens is not None:
@@ -81,7 +80,8 @@ def token_logprobs_reference(logits: Tensor, tokens: Tensor | None = None, *,
 
 def distillation_loss_reference(logits: Tensor, teacher_logprobs: Tensor, teacher_tokens: Tensor, *,
                                 temperature: float = 1.0, tail: bool = False) -> Tensor:
-    logq = _scaled_log_softmax(logits, temperature)
+    z = _scaled(logits, temperature)
+    logq = torch.log_softmax(z, dim=-1)
     tokens = teacher_tokens.long()
     present = tokens >= 0
     inside = present & (tokens < logits.shape[-1])
@@ -102,7 +102,9 @@ def distillation_loss_reference(logits: Tensor, teacher_logprobs: Tensor, teache
         listed.scatter_add_(-1, at, inside.int())
         rest = 1.0 - p.sum(dim=-1)
         some_rest = (rest > LEAST_REST) | rest.isnan()
-        outside = torch.logsumexp(logq.masked_fill(listed > 0, -math.inf), dim=-1)
+        # (from z, so that the denominator keeps its gradient where nothing is outside)
+        outside = torch.logsumexp(z.masked_fill(listed > 0, -math.inf), dim=-1)
+        outside = outside - torch.logsumexp(z, dim=-1)
         outside = torch.where(some_rest, outside, zero)
         rest = torch.where(some_rest, rest, zero + 1.0)
         loss = loss + torch.where(some_rest, rest * (rest.log() - outside), zero)

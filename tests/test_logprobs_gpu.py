@@ -569,3 +569,109 @@ def test_refusals_on_cuda():
     none = ops.linear_token_logprobs(torch.zeros(0, 16, device="cuda").bfloat16(),
                                      torch.zeros(9, 16, device="cuda").bfloat16(), entropy=True)
     assert none.entropy.shape == (0,)
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(3, 8, 1), (5, 24, 7), (2, 8, 257), (257, 72, 300), (129, 1096, 129)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_linear_forms_at_edge_sizes(rows, width, vocab, tail):
+    """One-token vocabularies, widths below and beside the 64-wide steps, one row past a tile."""
+    from ohara_b200 import ops
+    from ohara_b200.ops.logprobs import distillation_loss_reference, token_logprobs_reference
+
+    torch.manual_seed(vocab)
+    hidden = torch.randn(rows, width, device="cuda").bfloat16().requires_grad_()
+    weight = (2 * torch.randn(vocab, width, device="cuda") / width**0.5).bfloat16().requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), device="cuda")
+    k = min(3, vocab)
+    logp, ids = _list_of((rows,), vocab, k)
+    ids[0] = -1
+    wide = [t.detach().double().requires_grad_() for t in (hidden, weight)]
+    logits = wide[0] @ wide[1].T
+    got = ops.linear_token_logprobs(hidden, weight, tokens, entropy=True)
+    loss = ops.linear_distillation_loss(hidden, weight, logp, ids, tail=tail)
+    want = token_logprobs_reference(logits, tokens, entropy=True)
+    ref = distillation_loss_reference(logits, logp.double(), ids, tail=tail)
+    terms = (wide[0].detach().abs() @ wide[1].detach().abs().T).max().item()
+    atol = 4 * _slack(vocab) + 8 * terms * width**0.5 * 2.0**-24
+    _close(got.logprobs, want.logprobs, atol, 16 * 2.0**-24, "logprobs")
+    _close(got.entropy, want.entropy, 2 * atol, 16 * 2.0**-24, "entropy")
+    _close(loss, ref, 2 * atol + 40 * (k + 2) * 2.0**-24, 16 * 2.0**-24, "loss")
+    have = torch.autograd.grad([got.logprobs, loss], [hidden, weight], [torch.ones_like(loss)] * 2)
+    wanted = torch.autograd.grad([want.logprobs, ref], wide, [torch.ones_like(ref)] * 2)
+    for a, b in zip(have, wanted):
+        # two operators' gradients, each rounded to bf16 with its inputs, and their sum: 3 roundings of
+        # magnitudes that the sum may cancel, so against the larger of the parts
+        assert (a.double() - b).norm() <= 6 * 2.0**-9 * max(b.norm(), 0.05 * rows**0.5)
+
+
+def test_linear_gradients_one_at_a_time_and_of_nothing():
+    from ohara_b200 import ops
+
+    torch.manual_seed(11)
+    hidden = torch.randn(2, 40, 64, device="cuda").bfloat16()
+    weight = torch.randn(600, 64, device="cuda").bfloat16()
+    tokens = torch.randint(0, 600, (2, 40), device="cuda", dtype=torch.int32)
+
+    def grads(h, w):
+        leaves = [t for t in (h, w) if t.requires_grad]
+        got = ops.linear_token_logprobs(h, w, tokens, ignore_index=7)
+        return torch.autograd.grad(got.logprobs.sum(), leaves)
+
+    both = grads(hidden.clone().requires_grad_(), weight.clone().requires_grad_())
+    (only_h,) = grads(hidden.clone().requires_grad_(), weight)
+    (only_w,) = grads(hidden, weight.clone().requires_grad_())
+    assert torch.equal(both[0], only_h) and torch.equal(both[1], only_w)
+    # rows that are strided, expanded or not aligned are laid out for the product first
+    wide = torch.randn(40, 80, device="cuda").bfloat16()
+    for h in (wide[:, 3:67], wide[:, :64], wide[:1, :64].expand(40, 64), wide.t()[:64].t()):
+        got = ops.linear_token_logprobs(h, weight, tokens[0])
+        want = ops.linear_token_logprobs(h.contiguous(), weight, tokens[0])
+        assert torch.equal(got.logprobs, want.logprobs)
+    none = torch.zeros(0, 64, device="cuda").bfloat16().requires_grad_()
+    w = weight.clone().requires_grad_()
+    loss = ops.linear_distillation_loss(none, w, torch.zeros(0, 2, device="cuda"),
+                                        torch.zeros(0, 2, device="cuda", dtype=torch.long))
+    d_none, d_w = torch.autograd.grad(loss.sum(), [none, w])
+    assert d_none.shape == (0, 64) and not d_w.any()
+
+
+def test_hidden_state_forms_captured_and_replayed():
+    from ohara_b200 import ops
+
+    torch.manual_seed(12)
+    weight = torch.randn(1003, 128, device="cuda").bfloat16().requires_grad_()
+    hidden = torch.randn(33, 128, device="cuda").bfloat16().requires_grad_()
+    tokens = torch.randint(0, 1003, (33,), device="cuda")
+    logp, ids = _list_of((33,), 1003, 5)
+    g = torch.ones(33, device="cuda")
+
+    def step(h):
+        got = ops.linear_token_logprobs(h, weight, tokens, entropy=True)
+        loss = ops.linear_distillation_loss(h, weight, logp, ids, tail=True)
+        return (got.logprobs, got.entropy, loss,
+                *torch.autograd.grad([got.logprobs, got.entropy, loss], [h, weight], [g, g, g]))
+
+    step(hidden)                                  # sets the kernels up
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(hidden)
+    for _ in range(2):
+        fresh = torch.randn(33, 128, device="cuda").bfloat16()
+        hidden.data.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(fresh.requires_grad_())):
+            assert torch.equal(a, b)
+
+
+def test_gradient_keeps_the_layout_of_a_padded_vocabulary():
+    from ohara_b200 import ops
+
+    leaf = torch.randn(6, 1024, device="cuda").bfloat16().requires_grad_()
+    x = leaf[:, :1001]
+    got = ops.token_logprobs(x, torch.zeros(6, dtype=torch.long, device="cuda"))
+    (d,) = torch.autograd.grad(got.logprobs.sum(), x, retain_graph=True)
+    assert d.stride() == x.stride() and d.shape == x.shape
+    (whole,) = torch.autograd.grad(got.logprobs.sum(), leaf)
+    assert torch.equal(whole[:, :1001], d) and not whole[:, 1001:].any()
