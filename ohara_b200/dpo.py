@@ -23,6 +23,17 @@ def sequence_logps(logits: Tensor, labels: Tensor, ignore_index: int = IGNORE_IN
     return (picked.squeeze(-1) * keep).sum(dim=-1)
 
 
+def linear_sequence_logps(hidden: Tensor, weight: Tensor, labels: Tensor,
+                          ignore_index: int = IGNORE_INDEX) -> Tensor:
+    """:func:`sequence_logps` from final hidden states ``(B, T, width)`` and the output projection
+    ``(V, width)``: summed in fp32 over the positions that are not masked, without the ``(B, T, V)``
+    logits (:func:`ohara_b200.ops.linear_token_logprobs`)."""
+    from ohara_b200 import ops
+
+    found = ops.linear_token_logprobs(hidden, weight, labels, ignore_index=ignore_index)
+    return found.logprobs.sum(dim=-1)
+
+
 def _margin(pi_win: Tensor, pi_lose: Tensor, ref_win: Tensor, ref_lose: Tensor) -> Tensor:
     return (pi_win - pi_lose) - (ref_win - ref_lose)
 

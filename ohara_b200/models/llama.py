@@ -471,6 +471,35 @@ class Llama(nn.Module):
         self._release_after_inference()
         return loss
 
+    def _whole_head(self) -> Tensor:
+        """The output projection, for the operators that work from hidden states."""
+        weight = self.vocab_proj.weight
+        if hasattr(weight, "tensor_parallel_dim"):
+            raise NotImplementedError("a vocabulary-sharded head (mlp_and_head plan) gives no "
+                                      "log-probabilities over the whole vocabulary")
+        if getattr(self, "_param_sharding", None) is not None:
+            raise NotImplementedError("parameters that are sharded per block are released before the "
+                                      "backward pass of this loss needs them again")
+        return weight
+
+    def token_logprobs(self, x: Tensor, tokens: Tensor | None = None, *, temperature: float = 1.0,
+                       entropy: bool = False, top: int = 0, ignore_index: int = -100):
+        """Log-probabilities of ``tokens (B, T)`` at the positions of ``x (B, T)`` (so ``tokens`` are
+        ``x`` moved on by one for the next token), entropies and the most likely tokens, without a
+        logits tensor (:func:`ohara_b200.ops.linear_token_logprobs`). The inputs of preference losses;
+        with ``top`` on a teacher, of :meth:`distillation_loss`."""
+        weight = self._whole_head()
+        return ops.linear_token_logprobs(self.forward_hidden(x), weight, tokens, temperature=temperature,
+                                         entropy=entropy, top=top, ignore_index=ignore_index)
+
+    def distillation_loss(self, x: Tensor, teacher_logprobs: Tensor, teacher_tokens: Tensor, *,
+                          temperature: float = 1.0, tail: bool = False) -> Tensor:
+        """Divergence ``(B, T)`` from a teacher's list at every position, without a logits tensor
+        (:func:`ohara_b200.ops.linear_distillation_loss`). MoE auxiliary losses are not added."""
+        weight = self._whole_head()
+        return ops.linear_distillation_loss(self.forward_hidden(x), weight, teacher_logprobs,
+                                            teacher_tokens, temperature=temperature, tail=tail)
+
     def auxiliary_loss(self) -> Tensor | None:
         terms = [
             layer.ff.aux_loss

@@ -175,3 +175,48 @@ def test_empty_batches():
     got = ops.token_logprobs(x, torch.zeros(0, dtype=torch.long), entropy=True, top=2)
     assert got.logprobs.shape == (0,) and got.top_tokens.shape == (0, 2)
     assert ops.distillation_loss(x, torch.zeros(0, 3), torch.zeros(0, 3, dtype=torch.long)).shape == (0,)
+
+
+# -- where the framework uses them -------------------------------------------------------------------
+def _tiny_llama(seed=0):
+    from ohara_b200.models.llama import Config, Llama
+
+    torch.manual_seed(seed)
+    return Llama(Config(vocab_size=50, max_sequence_length=16, hidden_size=16, intermediate_size=32,
+                        num_attention_heads=2, num_key_value_heads=1, num_hidden_layers=1, dropout=0.0))
+
+
+def test_a_model_distils_from_another_and_gives_preference_inputs():
+    from ohara_b200.dpo import dpo_loss_from_logps, linear_sequence_logps, sequence_logps
+
+    student, teacher = _tiny_llama(0), _tiny_llama(1)
+    ids = torch.randint(0, 50, (2, 9))
+    x, labels = ids[:, :-1], ids[:, 1:].clone()
+    labels[0, :3] = -100
+    logits = student(x)
+    got = student.token_logprobs(x, labels, entropy=True)
+    want = torch.log_softmax(logits, -1)
+    torch.testing.assert_close(got.logprobs[1], want[1].gather(-1, labels[1][:, None])[:, 0])
+    assert not got.logprobs[0, :3].any() and got.entropy.shape == (2, 8)
+    summed = linear_sequence_logps(student.forward_hidden(x), student.vocab_proj.weight, labels)
+    torch.testing.assert_close(summed, sequence_logps(logits, labels))
+    losses, _ = dpo_loss_from_logps(summed[0], summed[1], summed[0].detach(), summed[1].detach(), 0.1)
+    with torch.no_grad():
+        listed = teacher.token_logprobs(x, top=5, temperature=2.0)
+    loss = student.distillation_loss(x, listed.top_logprobs, listed.top_tokens, temperature=2.0, tail=True)
+    torch.testing.assert_close(loss, ops.distillation_loss(logits, listed.top_logprobs, listed.top_tokens,
+                                                           temperature=2.0, tail=True))
+    (losses + loss.sum()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in student.parameters())
+
+
+def test_a_sharded_head_is_refused():
+    model = _tiny_llama()
+    model.vocab_proj.weight.tensor_parallel_dim = 0
+    with pytest.raises(NotImplementedError, match="vocabulary-sharded"):
+        model.token_logprobs(torch.zeros(1, 2, dtype=torch.long), entropy=True)
+    other = _tiny_llama()
+    other._param_sharding = object()
+    with pytest.raises(NotImplementedError, match="released"):
+        other.distillation_loss(torch.zeros(1, 2, dtype=torch.long), torch.zeros(1, 2, 1),
+                                torch.zeros(1, 2, 1, dtype=torch.long))
