@@ -12,6 +12,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -48,6 +49,20 @@ def _nvcc() -> str:
     if not found:
         raise RuntimeError("nvcc not found; cannot build the ohara_b200 CUDA extension")
     return found
+
+
+def _host_compiler() -> str:
+    """``$CXX`` if it links the shared C++ runtime, else the system's ``g++``. A compiler that only has the
+    static runtime gives the extension a second copy of it beside libtorch's, and the first C++ exception
+    that crosses the two (any refused argument) ends the process."""
+    for candidate in (os.environ.get("CXX"), shutil.which("g++"), shutil.which("c++")):
+        if not candidate:
+            continue
+        proc = subprocess.run([candidate, "-print-file-name=libstdc++.so"], capture_output=True, text=True)
+        if proc.returncode == 0 and os.path.isabs(proc.stdout.strip()):
+            return candidate
+    warnings.warn("no C++ compiler with a shared libstdc++ found: refused arguments may end the process")
+    return os.environ.get("CXX", "g++")
 
 
 def _torch_flags() -> tuple[list[str], list[str]]:
@@ -87,6 +102,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     """Compile every ``csrc/*.cu`` / ``*.cpp`` for sm_100a and link ``_C``. Returns the .so path."""
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     nvcc = _nvcc()
+    cxx = _host_compiler()
     torch_cflags, torch_libs = _torch_flags()
     header_mtime = _newest_header_mtime()
     sources = sorted(SRC_DIR.glob("*.cu")) + sorted(SRC_DIR.glob("*.cpp"))
@@ -108,7 +124,6 @@ def build(verbose: bool = False, force: bool = False) -> Path:
                 cmd.insert(1, "-Xptxas")
                 cmd.insert(2, "-v")
         else:
-            cxx = os.environ.get("CXX", "g++")
             cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
             cmd = [
                 cxx,
@@ -140,7 +155,6 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     target = ext_path()
     relink = bool(jobs) or not target.exists()
     if relink:
-        cxx = os.environ.get("CXX", "g++")
         cmd = [cxx, "-shared", "-o", str(target), *[str(o) for o in objects], *torch_libs]
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:

@@ -529,7 +529,7 @@ token_logprobs_kernel(const RowsView view, const TokenLogprobsArgs p) {
   // the warp has noted
   float best = -INFINITY, least_x = -INFINITY;
   int best_at = -1, least_at = 0x7fffffff, noted = 0, refresh_at = 0x7fffffff;
-  const BoundPlan plan = bound_plan<THREADS>(top);
+  const BoundPlan plan = TOP ? bound_plan<THREADS>(top) : BoundPlan{1, 1};
   using V = VectorCode<T>;
   using Code = typename V::Code;
   const int shift = V::shift_for(sl.v1);

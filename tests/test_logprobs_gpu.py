@@ -227,7 +227,7 @@ def test_rows_that_defeat_the_candidate_bound(vocab, top, dtype):
     x = torch.stack([torch.zeros(vocab, device="cuda"), ramp * 2.0**-10, -ramp * 2.0**-10, block,
                      torch.full((vocab,), -math.inf, device="cuda"), (ramp * 37) % 101])
     x[4, vocab - 2:] = 1.0
-    for repeat in (1, 80):                    # a cluster per row; one block per row
+    for repeat in (1, 80, 170):               # a cluster per row; blocks of 256 and of 128 threads
         _check(x.to(dtype).repeat(repeat, 1), None, entropy=False, top=top, backward=False)
 
 
@@ -675,3 +675,32 @@ def test_gradient_keeps_the_layout_of_a_padded_vocabulary():
     assert d.stride() == x.stride() and d.shape == x.shape
     (whole,) = torch.autograd.grad(got.logprobs.sum(), leaf)
     assert torch.equal(whole[:, :1001], d) and not whole[:, 1001:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_top_list_of_a_vocabulary_beyond_the_short_positions(dtype):
+    """Past 2^19 16-bit logits a vector's position no longer fits the short code: ties, masked rows."""
+    torch.manual_seed(13)
+    vocab = 1_200_003
+    x = _logits(3, vocab, dtype)
+    x[1, 50:] = -math.inf
+    x[2] = 0.25
+    for repeat in (1, 100):
+        _check(x.repeat(repeat, 1), None, entropy=False, top=100, backward=False)
+
+
+def test_tail_marks_of_a_large_vocabulary():
+    from ohara_b200 import ops
+
+    torch.manual_seed(14)
+    rows, vocab = 297, 300_001                # 75 KB of marks per block
+    x = _logits(rows, vocab, torch.float32)
+    scores = torch.log_softmax(torch.randn(rows, 9, device="cuda"), -1)[:, :-1].contiguous()
+    ids = torch.randint(0, vocab, (rows, 8), device="cuda")
+    ids[:, 0] = vocab - 1
+    _check_distill(x, scores, ids, tail=True)
+    # more marks than a block has room for: refused before anything is launched
+    huge = torch.zeros(1, 1_700_000, device="cuda").bfloat16().expand(rows, -1)
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.distillation_loss(huge, scores, ids, tail=True)
+    assert torch.isfinite(ops.distillation_loss(huge, scores, ids)).all()
