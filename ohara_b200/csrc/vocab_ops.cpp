@@ -1,7 +1,7 @@
 // Log-probabilities and distillation over the vocabulary for torch tensors: argument checks, outputs and
 // workspaces from torch's caching allocator (stream-ordered, so that calls on several streams and
 // captured graphs share nothing), and the autograd nodes. The nodes are C++ because a small batch is
-// bound by the host: a Python node costs about 35 us more per forward and backward pass (4 x 8192).
+// bound by the host: a forward and backward pass of 4 x 8192 takes 59 us, with Python nodes it took 86.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
