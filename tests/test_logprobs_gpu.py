@@ -503,7 +503,7 @@ def test_another_stream_and_two_captured_graphs():
             got = ops.token_logprobs(buf, ids, entropy=True, top=8)
             d = torch.autograd.grad(got.logprobs, buf, grad)[0]
         graphs.append(graph)
-        outs.append((*got, d))
+        outs.append([t.detach() for t in (*got, d)])
     for attempt in range(2):
         fresh = [_logits(4, 50304, torch.bfloat16) for _ in graphs]
         for buf, new in zip(inputs, fresh):
@@ -655,7 +655,7 @@ def test_hidden_state_forms_captured_and_replayed():
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out = step(hidden)
+        out = [t.detach() for t in step(hidden)]   # no autograd graph outlives the capture
     for _ in range(2):
         fresh = torch.randn(33, 128, device="cuda").bfloat16()
         hidden.data.copy_(fresh)
@@ -704,3 +704,22 @@ def test_tail_marks_of_a_large_vocabulary():
     with pytest.raises(RuntimeError, match="too large"):
         ops.distillation_loss(huge, scores, ids, tail=True)
     assert torch.isfinite(ops.distillation_loss(huge, scores, ids)).all()
+
+
+def test_a_single_row_without_leading_dimensions():
+    from ohara_b200 import ops
+
+    x = torch.randn(300, device="cuda", requires_grad=True)
+    token = torch.tensor(7, device="cuda")
+    got = _check(x, token, top=3)
+    assert got.logprobs.shape == () and got.top_tokens.shape == (3,)
+    _check_distill(x, *_list_of((), 300, 4), tail=True)
+    hidden = torch.randn(64, device="cuda").bfloat16().requires_grad_()
+    weight = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_()
+    alone = ops.linear_token_logprobs(hidden, weight, token, entropy=True)
+    d = torch.autograd.grad([alone.logprobs, alone.entropy], [hidden, weight])
+    rows = hidden.detach()[None].clone().requires_grad_()
+    batch = ops.linear_token_logprobs(rows, weight, token[None], entropy=True)
+    e = torch.autograd.grad([batch.logprobs.sum(), batch.entropy.sum()], [rows, weight])
+    assert alone.logprobs.shape == () and torch.equal(alone.logprobs, batch.logprobs[0])
+    assert torch.equal(d[0], e[0][0]) and torch.equal(d[1], e[1])
